@@ -102,7 +102,7 @@ def _fp8_group_scales(y):
     """(R, ceil(C / 128)) scales amax / 448, 1 where a group is all zeros."""
     groups = -(-y.shape[1] // GROUP)
     amax = _pad_cols(y, groups * GROUP).view(y.shape[0], groups, GROUP).abs().amax(dim=2)
-    return torch.where(amax > 0, amax / E4M3_MAX, torch.ones_like(amax))
+    return torch.where(amax > 0, amax / torch.full_like(amax, E4M3_MAX), torch.ones_like(amax))
 
 
 def _spread(scales, block, cols):
@@ -123,10 +123,15 @@ def _fp4_blocks(x, fmt, tensor_scale):
         q = _e2m1_round(blocks / scale.unsqueeze(2))
         return (e + 127).to(torch.uint8), (q * scale.unsqueeze(2)).view(rows, cols), None
     blocks = x.view(rows, cols // 16, 16)
+    # Divisors are tensors: a division by a number multiplies by its rounded reciprocal on a GPU, which moves
+    # values that lie next to a border of the 8- or 4-bit grid.
     if tensor_scale is None:
         amax = x.abs().amax()
-        tensor_scale = torch.where(amax > 0, amax / (E4M3_MAX * E2M1_MAX), torch.ones_like(amax))
-    scale8 = (blocks.abs().amax(dim=2) / E2M1_MAX / tensor_scale).clamp(max=E4M3_MAX).to(torch.float8_e4m3fn)
+        tensor_scale = torch.where(amax > 0, amax / torch.full_like(amax, E4M3_MAX * E2M1_MAX), torch.ones_like(amax))
+    else:
+        tensor_scale = torch.full((), tensor_scale, device=x.device)
+    amax = blocks.abs().amax(dim=2)
+    scale8 = (amax / torch.full_like(amax, E2M1_MAX) / tensor_scale).clamp(max=E4M3_MAX).to(torch.float8_e4m3fn)
     scale = scale8.float()
     denom = (scale * tensor_scale).unsqueeze(2)
     y = torch.where(denom > 0, blocks / torch.where(denom > 0, denom, torch.ones_like(denom)),
@@ -236,9 +241,8 @@ def prepare(case, seed):
             if fmt == "nvfp4" else None
         w = torch.randn(n, k, generator=g, device="cuda") * 0.02
         scales, values, w_scale = _fp4_blocks(w, fmt, None)
-        block = 32 if fmt == "mxfp4" else 16
-        unit = _as_scale_values(scales, fmt).float()
-        q = torch.where(_spread(unit, block, k) > 0, values / _spread(unit, block, k), 0.0)
+        unit = _spread(_as_scale_values(scales, fmt).float(), 32 if fmt == "mxfp4" else 16, k)
+        q = torch.where(unit > 0, values / unit, 0.0)
         s["w"], s["sw"], s["w_scale"] = _pack_e2m1(q), scales, None if w_scale is None else float(w_scale)
         if own:
             from gb300_microbench_b200 import lowp, quantize
