@@ -34,6 +34,7 @@ BB_ERR_INTERNAL = 6
 
 BB_DTYPE_BF16 = 1
 BB_DTYPE_F32 = 2
+BB_DTYPE_F16 = 3
 
 BB_VARIANT_NONPERSISTENT_1CTA = 0
 BB_VARIANT_PERSISTENT_1CTA = 1
@@ -98,9 +99,14 @@ class LowpInfo(ctypes.Structure):
     def as_dict(self) -> dict:
         return {name: int(getattr(self, name)) for name, _ in self._fields_ if name != "reserved"}
 
+    def as_linear_dict(self) -> dict:
+        return {**self.as_dict(), "few_rows": int(self.reserved[0]), "k_splits": int(self.reserved[1])}
+
 
 BB_LOWP_NVFP4 = 1
 BB_LOWP_FP8_BLOCK128 = 2
+BB_LOWP_MXFP4 = 3
+BB_LOWP_FP8_GROUP128 = 4
 
 # Every symbol include/b200bench.h declares, with (restype, argtypes).
 BENCH_SIGNATURES: dict[str, tuple] = {
@@ -142,6 +148,23 @@ BENCH_SIGNATURES: dict[str, tuple] = {
     "bb_lowp_synchronize": (c_int, [c_void_p]),
     "bb_lowp_launches": (c_int64, [c_void_p]),
     "bb_lowp_destroy": (c_int, [c_void_p]),
+    "bb_linear_scale_bytes": (c_int64, [c_int, c_int, c_int64, c_int64]),
+    "bb_linear_plan_create": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
+                                      c_void_p, c_float, c_void_p, c_float, c_void_p, c_void_p, c_int, c_int64,
+                                      c_void_p, POINTER(c_void_p), POINTER(LowpInfo)]),
+    "bb_linear_execute_n": (c_int, [c_void_p, c_int]),
+    "bb_linear_synchronize": (c_int, [c_void_p]),
+    "bb_linear_launches": (c_int64, [c_void_p]),
+    "bb_linear_destroy": (c_int, [c_void_p]),
+    "bb_fp4_quant_plan_create": (c_int, [c_int, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p, c_void_p,
+                                         c_float, c_void_p, c_void_p, c_int64, c_void_p, POINTER(c_void_p)]),
+    "bb_rmsnorm_fp8_plan_create": (c_int, [c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p,
+                                           c_int64, c_void_p, c_int, c_float, c_void_p, c_int64, c_void_p, c_int64,
+                                           c_void_p, POINTER(c_void_p)]),
+    "bb_quant_execute_n": (c_int, [c_void_p, c_int]),
+    "bb_quant_synchronize": (c_int, [c_void_p]),
+    "bb_quant_launches": (c_int64, [c_void_p]),
+    "bb_quant_destroy": (c_int, [c_void_p]),
 }
 
 class CmpInfo(ctypes.Structure):

@@ -35,6 +35,8 @@ BENCH_SOURCES = [
     "gemm_capi.cu",
     "gemm_noalloc.cu",
     "gemm_lowp.cu",
+    "lowp_linear.cu",
+    "quantize.cu",
     "copy_kernels.cu",
     "umma_probe.cu",
 ]

@@ -55,4 +55,18 @@ struct DeviceInfo {
 };
 int query_device(DeviceInfo* info);
 
+// Makes the plan's device current for a launch, and the caller's again after it.
+struct DeviceGuard {
+  int before = -1;
+  cudaError_t status;
+  explicit DeviceGuard(int device) {
+    status = cudaGetDevice(&before);
+    if (status == cudaSuccess && before != device) status = cudaSetDevice(device);
+    else before = -1;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
 }  // namespace bb

@@ -9,13 +9,24 @@ with tensor_scale = amax(|x|) / (448 * 6) and block scale = amax(block) / 6 /
 tensor_scale rounded to E4M3, values rounded to nearest (ties to even) on
 the E2M1 grid {0, 0.5, 1, 1.5, 2, 3, 4, 6}.
 
+MXFP4: E2M1 values with one E8M0 scale per 32 consecutive K elements,
+scale = 2^(floor(log2 amax(block)) - 2), no tensor scale; a block that holds
+a NaN or an infinity has the scale NaN.
+
 FP8 block-scaled: E4M3 values with one FP32 scale per 128 x 128 block,
-scale = amax(block) / 448.
+scale = amax(block) / 448. FP8 group-scaled (activations): one FP32 scale
+per row and 128 consecutive K elements.
 
 The kernels read the NVFP4 block scales in "scale atoms": for each group of
 128 rows and each 64 K elements (4 scales per row), 512 bytes in which the
 scale j of row r sits at byte (r % 32) * 16 + (r // 32) * 4 + j. One atom is
 what one ``tcgen05.cp.32x128b.warpx4`` moves into TMEM for one K = 64 MMA.
+MXFP4 block scales use the same atoms, each covering 128 K elements.
+
+:class:`LowpGemmPlan` is the GEMM of two operands of aligned extents;
+:class:`LowpLinearPlan` is a linear layer's product, for any number of rows
+(one token upwards) and any output width. :mod:`.quantize` has the
+quantisers as kernels; the functions here are their definitions in torch.
 """
 from __future__ import annotations
 
@@ -50,15 +61,21 @@ def e2m1_decode(codes: torch.Tensor) -> torch.Tensor:
     return torch.where((codes & 8) != 0, -mag, mag)
 
 
-def nvfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, float]:
+def nvfp4_quantize(x: torch.Tensor, tensor_scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor, float]:
     """x (R, K) float32, K % 16 == 0 -> (packed (R, K/2) uint8,
-    block scales (R, K/16) uint8 E4M3 bits, tensor scale float)."""
+    block scales (R, K/16) uint8 E4M3 bits, tensor scale float). The tensor
+    scale is found from x unless one is given (a calibrated one)."""
     if x.dim() != 2 or x.shape[1] % 16:
         raise ValueError("x must be (R, K) with K a multiple of 16")
     x = x.float()
     r, k = x.shape
-    amax = float(x.abs().max())
-    gscale = amax / (E4M3_MAX * E2M1_MAX) if amax > 0 else 1.0
+    if tensor_scale is None:
+        amax = float(x.abs().max())
+        gscale = amax / (E4M3_MAX * E2M1_MAX) if amax > 0 else 1.0
+        if torch.tensor(gscale, dtype=torch.float32) == 0:  # below FP32: everything rounds to zero
+            gscale = 1.0
+    else:
+        gscale = float(tensor_scale)
     blocks = x.view(r, k // 16, 16)
     bs = (blocks.abs().amax(dim=2) / E2M1_MAX / gscale).clamp(max=E4M3_MAX)
     bs8 = bs.to(torch.float8_e4m3fn)
@@ -81,6 +98,37 @@ def nvfp4_dequantize(packed: torch.Tensor, scales: torch.Tensor, gscale: float) 
     return vals * s * gscale
 
 
+def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x (R, K) float32, K % 32 == 0 -> (packed (R, K/2) uint8, block scales
+    (R, K/32) uint8 E8M0 bits)."""
+    if x.dim() != 2 or x.shape[1] % 32:
+        raise ValueError("x must be (R, K) with K a multiple of 32")
+    x = x.float()
+    r, k = x.shape
+    blocks = x.view(r, k // 32, 32)
+    amax = blocks.abs().amax(dim=2)
+    # floor(log2 amax) - 2 + 127: amax's biased exponent less 2, not below 0.
+    e = (amax.view(torch.int32) >> 23) & 0xFF
+    bits = torch.where(e == 255, 255, (e - 2).clamp(min=0)).to(torch.uint8)
+    y = blocks * mxfp4_scale_values(254 - bits.clamp(max=253)).unsqueeze(2)  # 1 / scale, exactly
+    y = torch.where((bits == 255).unsqueeze(2), torch.zeros_like(y), y)
+    codes = _e2m1_codes(y).view(r, k)
+    return (codes[:, 0::2] | (codes[:, 1::2] << 4)).contiguous(), bits
+
+
+def mxfp4_scale_values(bits: torch.Tensor) -> torch.Tensor:
+    """E8M0 bytes -> FP32: 2^(byte - 127), NaN for 255."""
+    b = bits.to(torch.int32)
+    f = torch.where(b == 0, 1 << 22, b << 23)  # 2^-127 lies below the normal numbers
+    return torch.where(b == 255, 0x7FC00000, f).to(torch.int32).view(torch.float32)
+
+
+def mxfp4_dequantize(packed: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    r, kh = packed.shape
+    codes = torch.stack((packed & 0xF, packed >> 4), dim=2).view(r, kh * 2)
+    return e2m1_decode(codes) * mxfp4_scale_values(scales).repeat_interleave(32, dim=1)
+
+
 def pack_scale_atoms(scales: torch.Tensor) -> torch.Tensor:
     """(R, K/16) scale bytes -> (ceil(R/128), ceil(K/64), 512) atoms (rows and
     K padded with zero scales)."""
@@ -93,6 +141,21 @@ def pack_scale_atoms(scales: torch.Tensor) -> torch.Tensor:
     t = padded.view(rb, 4, 32, kg, 4)
     # atom byte = (r % 32) * 16 + (r // 32) * 4 + j  ->  order [rb][kg][r%32][r//32][j]
     return t.permute(0, 3, 2, 1, 4).contiguous().view(rb, kg, 512)
+
+
+def unpack_scale_atoms(atoms: torch.Tensor, rows: int, width: int) -> torch.Tensor:
+    """The inverse of :func:`pack_scale_atoms`: (rows, width) scale bytes."""
+    rb, kg, _ = atoms.shape
+    t = atoms.view(rb, kg, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(rb * 128, kg * 4)
+    return t[:rows, :width].contiguous()
+
+
+def _extents(rows: int, k: int, step: int) -> tuple[int, int]:
+    rows, k = int(rows), int(k)
+    if rows < 0 or k <= 0 or k % step:
+        raise ValueError(f"rows must not be negative and K positive{f' and a multiple of {step}' if step > 1 else ''}: "
+                         f"got {rows} x {k}")
+    return rows, k
 
 
 def fp8_block_quantize(x: torch.Tensor, block: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
@@ -116,10 +179,35 @@ def fp8_block_dequantize(q: torch.Tensor, scale: torch.Tensor, block: int = 128)
     return v * s
 
 
+def fp8_group_quantize(x: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
+    """x (R, K) -> (E4M3 bits (R, K) uint8, FP32 scales (R, ceil(K/128)))
+    with scale = amax(group) / 448, 1 where that is 0."""
+    x = x.float()
+    r, k = x.shape
+    kb = -(-k // group)
+    blocks = torch.nn.functional.pad(x, (0, kb * group - k)).view(r, kb, group)
+    amax = blocks.abs().amax(dim=2)
+    scale = torch.where(amax == 0, torch.ones_like(amax), amax / torch.full_like(amax, E4M3_MAX))
+    q = (blocks / scale[:, :, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+    return q.view(r, kb * group)[:, :k].contiguous().view(torch.uint8), scale
+
+
+def fp8_group_dequantize(q: torch.Tensor, scale: torch.Tensor, group: int = 128) -> torch.Tensor:
+    v = q.view(torch.float8_e4m3fn).float()
+    return v * scale.repeat_interleave(group, 1)[:, : v.shape[1]]
+
+
 # ------------------------------------------------------------------ operands
 class Nvfp4Operand:
     """A quantised NVFP4 operand: packed E2M1 (R, K/2) bytes, scale atoms,
-    per-tensor FP32 scale."""
+    per-tensor FP32 scale.
+
+    One made by :meth:`empty` is filled by :class:`.quantize.Fp4QuantPlan`;
+    it keeps its scales as atoms only (``scales`` is None), and where its
+    tensor scale is found from the data that is the device tensor
+    ``tensor_scale_out`` (1,) and ``tensor_scale`` is None."""
+
+    tensor_scale_out: torch.Tensor | None = None
 
     def __init__(self, x: torch.Tensor):
         self.rows, self.k = x.shape
@@ -138,12 +226,124 @@ class Nvfp4Operand:
         op.atoms = pack_scale_atoms(op.scales)
         return op
 
+    @classmethod
+    def empty(cls, rows: int, k: int, device: str | torch.device = "cuda",
+              tensor_scale: float | None = None) -> "Nvfp4Operand":
+        """Buffers for a quantiser to fill, K a multiple of 32; ``tensor_scale``
+        None: to be found from the data."""
+        op = cls.__new__(cls)
+        op.rows, op.k = _extents(rows, k, 32)
+        op.data = torch.empty(rows, k // 2, dtype=torch.uint8, device=device)
+        op.scales = None
+        op.atoms = torch.empty(-(-rows // 128), -(-k // 64), 512, dtype=torch.uint8, device=device)
+        op.tensor_scale = None if tensor_scale is None else float(tensor_scale)
+        if tensor_scale is None:
+            op.tensor_scale_out = torch.ones(1, dtype=torch.float32, device=device)
+        return op
+
     def to(self, device) -> "Nvfp4Operand":
+        if self.scales is None:
+            op = Nvfp4Operand.__new__(Nvfp4Operand)
+            op.rows, op.k, op.scales, op.tensor_scale = self.rows, self.k, None, self.tensor_scale
+            op.data, op.atoms = self.data.to(device), self.atoms.to(device)
+            if self.tensor_scale_out is not None:
+                op.tensor_scale_out = self.tensor_scale_out.to(device)
+            return op
         op = Nvfp4Operand.from_parts(self.data.to(device), self.scales.to(device), self.tensor_scale)
         return op
 
     def dequantize(self) -> torch.Tensor:
-        return nvfp4_dequantize(self.data, self.scales, self.tensor_scale)
+        scales = unpack_scale_atoms(self.atoms, self.rows, self.k // 16) if self.scales is None else self.scales
+        gscale = self.tensor_scale_out if self.tensor_scale is None else self.tensor_scale
+        return nvfp4_dequantize(self.data, scales, gscale)
+
+
+class Mxfp4Operand:
+    """A quantised MXFP4 operand: packed E2M1 (R, K/2) bytes and E8M0 scales
+    (R, K/32) as scale atoms. One made by :meth:`empty` is filled by
+    :class:`.quantize.Fp4QuantPlan`."""
+
+    def __init__(self, x: torch.Tensor):
+        self.rows, self.k = x.shape
+        self.data, scales = mxfp4_quantize(x)
+        self.atoms = pack_scale_atoms(scales)
+
+    @classmethod
+    def from_parts(cls, data: torch.Tensor, scales: torch.Tensor) -> "Mxfp4Operand":
+        """An operand from already-encoded parts: packed E2M1 (R, K/2) bytes
+        and E8M0 scale bytes (R, K/32)."""
+        if data.dim() != 2 or data.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise ValueError("data and scales must be uint8, data (R, K/2)")
+        op = cls.__new__(cls)
+        op.rows, op.k = data.shape[0], data.shape[1] * 2
+        if tuple(scales.shape) != (op.rows, op.k // 32) or op.k % 32:
+            raise ValueError(f"scales {tuple(scales.shape)} do not fit data {tuple(data.shape)}: K must be a multiple "
+                             "of 32 with one scale per 32")
+        op.data, op.atoms = data.contiguous(), pack_scale_atoms(scales)
+        return op
+
+    @classmethod
+    def empty(cls, rows: int, k: int, device: str | torch.device = "cuda") -> "Mxfp4Operand":
+        """Buffers for a quantiser to fill, K a multiple of 32."""
+        op = cls.__new__(cls)
+        op.rows, op.k = _extents(rows, k, 32)
+        op.data = torch.empty(rows, k // 2, dtype=torch.uint8, device=device)
+        op.atoms = torch.empty(-(-rows // 128), -(-k // 128), 512, dtype=torch.uint8, device=device)
+        return op
+
+    def to(self, device) -> "Mxfp4Operand":
+        op = Mxfp4Operand.__new__(Mxfp4Operand)
+        op.rows, op.k, op.data, op.atoms = self.rows, self.k, self.data.to(device), self.atoms.to(device)
+        return op
+
+    def dequantize(self) -> torch.Tensor:
+        return mxfp4_dequantize(self.data, unpack_scale_atoms(self.atoms, self.rows, self.k // 32))
+
+
+class Fp8GroupOperand:
+    """Activations in FP8: E4M3 (R, K) bytes and one FP32 scale per row and 128
+    columns. ``scales`` is (R, ceil(K/128)) with the scales of one column
+    group side by side in memory (strides (1, R)), as the product reads them.
+    One made by :meth:`empty` is filled by :class:`.quantize.RmsNormFp8Plan`."""
+
+    def __init__(self, x: torch.Tensor):
+        self.rows, self.k = x.shape
+        self.data, scales = fp8_group_quantize(x)
+        self.scales = scales.t().contiguous().t()
+
+    @classmethod
+    def from_parts(cls, data: torch.Tensor, scales: torch.Tensor) -> "Fp8GroupOperand":
+        """From E4M3 values (uint8 or float8_e4m3fn (R, K)) and FP32 scales (R, ceil(K/128))."""
+        if data.dim() != 2 or data.dtype not in (torch.uint8, torch.float8_e4m3fn):
+            raise ValueError("data must be (R, K) uint8 or float8_e4m3fn")
+        op = cls.__new__(cls)
+        op.rows, op.k = data.shape
+        if tuple(scales.shape) != (op.rows, -(-op.k // 128)) or scales.dtype != torch.float32:
+            raise ValueError(f"scales {tuple(scales.shape)} {scales.dtype}: expected float32 "
+                             f"{(op.rows, -(-op.k // 128))}")
+        op.data = data.contiguous().view(torch.uint8)
+        op.scales = scales.t().contiguous().t()  # no copy where it is laid out so already
+        return op
+
+    @classmethod
+    def empty(cls, rows: int, k: int, device: str | torch.device = "cuda") -> "Fp8GroupOperand":
+        """Buffers for a quantiser to fill. (The product needs K a multiple of 16.)"""
+        op = cls.__new__(cls)
+        op.rows, op.k = _extents(rows, k, 1)
+        op.data = torch.empty(rows, k, dtype=torch.uint8, device=device)
+        op.scales = torch.empty(-(-k // 128), rows, dtype=torch.float32, device=device).t()
+        return op
+
+    @property
+    def values(self) -> torch.Tensor:
+        """The E4M3 values, (R, K) float8_e4m3fn (a view)."""
+        return self.data.view(torch.float8_e4m3fn)
+
+    def to(self, device) -> "Fp8GroupOperand":
+        return Fp8GroupOperand.from_parts(self.data.to(device), self.scales.to(device))
+
+    def dequantize(self) -> torch.Tensor:
+        return fp8_group_dequantize(self.data, self.scales)
 
 
 class Fp8BlockOperand:
@@ -311,6 +511,111 @@ class CublasLtLowpPlan:
     def close(self) -> None:
         if getattr(self, "_handle", None):
             self._lib.bb_cmp_destroy(self._handle)
+            self._handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# ------------------------------------------------------------------ linear layer
+_LINEAR_KINDS = {Nvfp4Operand: ("nvfp4", nat.BB_LOWP_NVFP4, Nvfp4Operand),
+                 Mxfp4Operand: ("mxfp4", nat.BB_LOWP_MXFP4, Mxfp4Operand),
+                 Fp8GroupOperand: ("fp8_group128", nat.BB_LOWP_FP8_GROUP128, Fp8BlockOperand)}
+_D_DTYPES = {torch.bfloat16: nat.BB_DTYPE_BF16, torch.float16: nat.BB_DTYPE_F16, torch.float32: nat.BB_DTYPE_F32}
+
+
+class LowpLinearPlan:
+    """D (M, N) = dequant(x) @ dequant(w)^T: the product of a linear layer with
+    quantised weights and activations, for any number of rows from one token
+    upwards and any N (bb_linear_plan_create of include/b200bench.h).
+
+    The kind follows from the operands: :class:`Nvfp4Operand` or
+    :class:`Mxfp4Operand` for both (K a multiple of 32), or
+    :class:`Fp8GroupOperand` activations with :class:`Fp8BlockOperand`
+    weights (K a multiple of 16). D is bfloat16, float16 or float32 with
+    unit column stride and row stride >= N; its bytes outside (M, N) are not
+    touched. Tensor scales found on the GPU (``tensor_scale_out``) are read there
+    at every run. The plan keeps its operands; x may be refilled between runs."""
+
+    def __init__(self, x, w, d: torch.Tensor, stream: torch.cuda.Stream | None = None):
+        if type(x) not in _LINEAR_KINDS:
+            raise ValueError(f"x is {type(x).__name__}; expected one of "
+                             f"{sorted(c.__name__ for c in _LINEAR_KINDS)}")
+        self.kind, kind, w_type = _LINEAR_KINDS[type(x)]
+        if type(w) is not w_type:
+            raise ValueError(f"{type(x).__name__} activations take {w_type.__name__} weights, got {type(w).__name__}")
+        if d.dtype not in _D_DTYPES:
+            raise ValueError("D must be bfloat16, float16 or float32")
+        self.m, self.n, self.k = x.rows, w.rows, x.k
+        if w.k != x.k or tuple(d.shape) != (self.m, self.n):
+            raise ValueError(f"shape mismatch: x ({x.rows}, {x.k}), w ({w.rows}, {w.k}), D {tuple(d.shape)}")
+        if (self.n > 1 and d.stride(1) != 1) or (self.m > 1 and d.stride(0) < self.n):
+            raise ValueError("D must have unit column stride and a row stride of at least N")
+        step = 16 if self.kind == "fp8_group128" else 32
+        if self.k % step:
+            raise ValueError(f"K = {self.k} must be a multiple of {step} for {self.kind}")
+        fp8 = self.kind == "fp8_group128"
+        sx, sw = (x.scales, w.scales) if fp8 else (x.atoms, w.atoms)
+        scale_devs = [None if fp8 else getattr(op, "tensor_scale_out", None) for op in (x, w)]
+        tensors = [x.data, w.data, sx, sw, d] + [t for t in scale_devs if t is not None]
+        if not all(t.is_cuda for t in tensors):
+            raise ValueError("operands and D must be CUDA tensors")
+        if len({t.device for t in tensors}) != 1:
+            raise ValueError(f"operands and D on {sorted({str(t.device) for t in tensors})}: all must be on one device")
+        row_bytes = self.k if fp8 else self.k // 2
+        for name, op in (("x", x), ("w", w)):
+            if not op.data.is_contiguous() or op.data.numel() * op.data.element_size() < op.rows * row_bytes:
+                raise ValueError(f"{name} data must be contiguous and hold {op.rows} x {row_bytes} bytes")
+        self._lib = nat.bench_lib()
+        sx_ld = self.m
+        if fp8:
+            if tuple(sx.shape) != (self.m, -(-self.k // 128)) or (self.m > 1 and sx.stride(0) != 1) or (
+                    sx.shape[1] > 1 and sx.stride(1) < self.m) or sx.dtype != torch.float32:
+                raise ValueError("x scales must be float32 (M, ceil(K/128)) with strides (1, >= M)")
+            sx_ld = sx.stride(1) if sx.shape[1] > 1 else max(self.m, 1)
+        for name, t, weights, rows in (("x", sx, 0, self.m), ("w", sw, 1, self.n)):
+            need = int(self._lib.bb_linear_scale_bytes(kind, weights, rows, self.k))
+            if not (fp8 and not weights) and (not t.is_contiguous() or t.numel() * t.element_size() < need):
+                raise ValueError(f"{name} scales must be contiguous and hold {need} bytes")
+        self.stream = stream if stream is not None else torch.cuda.current_stream(d.device)
+        if self.stream.device != d.device:
+            raise ValueError(f"stream on {self.stream.device}, tensors on {d.device}")
+        scales = [1.0 if fp8 or getattr(op, "tensor_scale", None) is None else op.tensor_scale for op in (x, w)]
+        self.x, self.w, self.d, self._keep = x, w, d, tensors
+        handle = ctypes.c_void_p()
+        info = nat.LowpInfo()
+        with torch.cuda.device(d.device):
+            nat.check("bb_linear_plan_create", self._lib.bb_linear_plan_create(
+                kind, self.m, self.n, self.k, x.data.data_ptr(), w.data.data_ptr(), sx.data_ptr(), sx_ld,
+                sw.data_ptr(), scales[0], None if scale_devs[0] is None else scale_devs[0].data_ptr(), scales[1],
+                None if scale_devs[1] is None else scale_devs[1].data_ptr(), d.data_ptr(), _D_DTYPES[d.dtype],
+                d.stride(0) if self.m > 1 else self.n, self.stream.cuda_stream, ctypes.byref(handle),
+                ctypes.byref(info)))
+        self._handle = handle
+        self.info = info.as_linear_dict()
+
+    @property
+    def flops(self) -> int:
+        return 2 * self.m * self.n * self.k
+
+    def run(self, iterations: int = 1) -> None:
+        """`iterations` back-to-back launches on the plan's stream (async)."""
+        nat.check("bb_linear_execute_n", self._lib.bb_linear_execute_n(self._handle, int(iterations)))
+
+    def synchronize(self) -> None:
+        """Waits for the stream; raises on a device-side wait timeout."""
+        nat.check("bb_linear_synchronize", self._lib.bb_linear_synchronize(self._handle))
+
+    @property
+    def launches(self) -> int:
+        return int(self._lib.bb_linear_launches(self._handle))
+
+    def close(self) -> None:
+        if getattr(self, "_handle", None):
+            self._lib.bb_linear_destroy(self._handle)
             self._handle = None
 
     def __del__(self):

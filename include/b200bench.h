@@ -58,7 +58,7 @@ BB_API const char* bb_status_name(int status);
  * reference configures at gemm_comparison/gemm_comparison.py:209-260 and
  * launches at gemm_comparison.py:2850-2867.
  */
-enum { BB_DTYPE_BF16 = 1, BB_DTYPE_F32 = 2 };
+enum { BB_DTYPE_BF16 = 1, BB_DTYPE_F32 = 2, BB_DTYPE_F16 = 3 };
 
 /* The three reference candidate slots (gemm_comparison.py:209-245) plus the
  * tuned configuration of this library. */
@@ -267,7 +267,7 @@ BB_API int64_t bb_kernel_launches(void);
  *   per 128 x 128 block; global_scale multiplies the result (1 for none).
  *   K must be a multiple of 128.
  * N must be a multiple of 8 and every buffer 16-byte aligned. */
-enum { BB_LOWP_NVFP4 = 1, BB_LOWP_FP8_BLOCK128 = 2 };
+enum { BB_LOWP_NVFP4 = 1, BB_LOWP_FP8_BLOCK128 = 2, BB_LOWP_MXFP4 = 3, BB_LOWP_FP8_GROUP128 = 4 };
 
 typedef struct bb_lowp_info {
   int64_t kind;
@@ -296,6 +296,69 @@ BB_API int bb_lowp_execute_n(bb_lowp_plan* plan, int iterations);
 BB_API int bb_lowp_synchronize(bb_lowp_plan* plan);
 BB_API int64_t bb_lowp_launches(const bb_lowp_plan* plan);
 BB_API int bb_lowp_destroy(bb_lowp_plan* plan);
+
+/* ====================================================== quantised linear layer
+ * D (M x N) = dequant(A) * dequant(B)^T for any number of rows, from one
+ * token to a prefill, and any N. No counterpart in the reference.
+ *
+ * BB_LOWP_NVFP4: as above, K a multiple of 32 (scale atoms padded with zero
+ *   scales to a multiple of 64 K elements).
+ * BB_LOWP_MXFP4: E2M1 values, one E8M0 scale (2^(byte - 127), 255 = NaN) per
+ *   32 K elements in the same 512-byte atoms: atom (rb * ceil(K/128) + kg),
+ *   scale j of its four covers K elements [128 kg + 32 j, + 32). K a multiple
+ *   of 32.
+ * BB_LOWP_FP8_GROUP128: A and B hold E4M3 bytes, K a multiple of 16. sfa is
+ *   FP32 [ceil(K/128)][sfa_ld], one scale per row and 128 K elements (sfa_ld >=
+ *   M), sfb FP32 [ceil(N/128)][ceil(K/128)], one per 128 x 128 block.
+ *
+ * The result is multiplied by scale_a * scale_b, each read on the device
+ * from scale_a_dev / scale_b_dev (FP32) where that is not NULL. A, B, sfa and
+ * sfb are 16-byte aligned (FP8's sfa: 4); D has row stride ldd >= N and its
+ * type's alignment. M = 0 is a valid plan that launches nothing. */
+typedef struct bb_linear_plan bb_linear_plan;
+/* Bytes of a scale operand: of the weights (weights != 0, rows = N) or of the
+ * activations (rows = M; FP8_GROUP128: with sfa_ld = rows), or -1. */
+BB_API int64_t bb_linear_scale_bytes(int kind, int weights, int64_t rows, int64_t k);
+/* info->reserved[0]: 1 when the kernel for few rows runs; [1]: its K splits. */
+BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, const void* a, const void* b,
+                                 const void* sfa, int64_t sfa_ld, const void* sfb, float scale_a,
+                                 const float* scale_a_dev, float scale_b, const float* scale_b_dev, void* d,
+                                 int d_dtype, int64_t ldd, void* stream, bb_linear_plan** plan, bb_lowp_info* info);
+BB_API int bb_linear_execute_n(bb_linear_plan* plan, int iterations);
+/* Waits for the plan's stream; BB_ERR_TIMEOUT if a device wait ran out. */
+BB_API int bb_linear_synchronize(bb_linear_plan* plan);
+BB_API int64_t bb_linear_launches(const bb_linear_plan* plan);
+BB_API int bb_linear_destroy(bb_linear_plan* plan);
+
+/* ====================================================== quantisers
+ * One plan type for both; no counterpart in the reference. rows = 0 is a valid
+ * plan that launches nothing. */
+typedef struct bb_quant_plan bb_quant_plan;
+/* x (rows x cols, row stride x_ld, cols a multiple of 32) to BB_LOWP_NVFP4 or
+ * BB_LOWP_MXFP4: E2M1 codes into data (rows x cols / 2 bytes) and scale atoms
+ * (padding rows and columns zero) into scales, as bb_linear_plan_create reads
+ * them. NVFP4 with tensor_scale_out == NULL uses tensor_scale; otherwise the
+ * tensor scale is max|x| / 2688 (1 where that is 0 in FP32 or NaN), found by a launch of its
+ * own and written to *tensor_scale_out (device). values (may be NULL, x's
+ * dtype, row stride values_ld) receives what the codes stand for. */
+BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t x_ld,
+                                    void* data, void* scales, float tensor_scale, float* tensor_scale_out,
+                                    void* values, int64_t values_ld, void* stream, bb_quant_plan** plan);
+/* h = x + residual rounded to x's dtype (residual NULL: h = x), stored to
+ * residual_out where that is not NULL (it may be residual or x); y = h *
+ * rsqrt(mean(h^2) + eps) * weight; q = E4M3 of y / s (row stride q_ld) with s =
+ * max|y| / 448 over each 128 columns (1 where that is 0), stored to
+ * scales[group * scales_ld + row]. cols up to 65536; weight is FP32 or of x's
+ * dtype. A row that holds a NaN or an infinity is NaN. */
+BB_API int bb_rmsnorm_fp8_plan_create(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t x_ld,
+                                      const void* residual, int64_t residual_ld, void* residual_out,
+                                      int64_t residual_out_ld, const void* weight, int weight_dtype, float eps,
+                                      void* q, int64_t q_ld, float* scales, int64_t scales_ld, void* stream,
+                                      bb_quant_plan** plan);
+BB_API int bb_quant_execute_n(bb_quant_plan* plan, int iterations);
+BB_API int bb_quant_synchronize(bb_quant_plan* plan);
+BB_API int64_t bb_quant_launches(const bb_quant_plan* plan);
+BB_API int bb_quant_destroy(bb_quant_plan* plan);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,255 @@
+"""The quantised linear layer's product (LowpLinearPlan) on the GPU: against
+64-bit products of the decoded operands, from one row to several tiles, at
+odd widths and K, into strided and differently typed D; and the layer as it is
+used, from the residual stream through quantiser and product."""
+import pytest
+import torch
+
+from gb300_microbench_b200 import lowp, quantize
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ["nvfp4", "mxfp4", "fp8"]
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+def _exact_operand(kind, rows, k, gen, weights):
+    """Small integers with power-of-two scales: every product and sum is exact in FP32."""
+    if kind == "fp8":
+        q = torch.randint(-15, 16, (rows, k), generator=gen).float().to(torch.float8_e4m3fn).view(torch.uint8)
+        kb = -(-k // 128)
+        s = torch.exp2(torch.randint(-1, 2, (-(-rows // 128) if weights else rows, kb), generator=gen).float())
+        return lowp.Fp8BlockOperand.from_parts(q, s) if weights else lowp.Fp8GroupOperand.from_parts(q, s)
+    codes = torch.randint(0, 256, (rows, k // 2), generator=gen, dtype=torch.uint8)
+    if kind == "mxfp4":
+        return lowp.Mxfp4Operand.from_parts(codes, torch.randint(126, 129, (rows, k // 32), generator=gen).to(torch.uint8))
+    bits = ((torch.randint(-1, 2, (rows, k // 16), generator=gen) + 7) << 3).to(torch.uint8)
+    return lowp.Nvfp4Operand.from_parts(codes, bits, 0.5 if weights else 2.0)
+
+
+def _quantised_operand(kind, rows, k, gen, weights):
+    x = torch.randn(rows, k, generator=gen) * torch.exp(torch.randn(k, generator=gen) * 0.3)
+    if kind == "fp8":
+        return lowp.Fp8BlockOperand(x) if weights else lowp.Fp8GroupOperand(x)
+    return lowp.Mxfp4Operand(x) if kind == "mxfp4" else lowp.Nvfp4Operand(x)
+
+
+def _decode(op):
+    if isinstance(op, lowp.Fp8BlockOperand):
+        s = op.scales.double().repeat_interleave(128, 0).repeat_interleave(128, 1)[:op.rows, :op.k]
+        return op.data.view(torch.float8_e4m3fn).double() * s
+    if isinstance(op, lowp.Fp8GroupOperand):
+        return op.values.double() * op.scales.double().repeat_interleave(128, 1)[:, :op.k]
+    if isinstance(op, lowp.Mxfp4Operand):
+        return lowp.mxfp4_dequantize(op.data, lowp.unpack_scale_atoms(op.atoms, op.rows, op.k // 32)).double()
+    g = op.tensor_scale if op.tensor_scale is not None else float(op.tensor_scale_out)
+    bits = lowp.unpack_scale_atoms(op.atoms, op.rows, op.k // 16)
+    return lowp.nvfp4_dequantize(op.data, bits, 1.0).double() * g
+
+
+def _run(x, w, dev, dtype=torch.bfloat16, d=None):
+    if d is None:
+        d = torch.full((x.rows, w.rows), float("nan"), dtype=dtype, device=dev)
+    plan = lowp.LowpLinearPlan(x.to(dev), w.to(dev), d)
+    plan.run()
+    plan.synchronize()
+    assert plan.launches >= (1 if x.rows else 0)
+    first = d.clone()
+    plan.run()
+    plan.synchronize()
+    assert torch.equal(first.view(torch.uint8), d.view(torch.uint8)) if d.is_contiguous() else torch.equal(first, d)
+    plan.close()
+    return d.cpu()
+
+
+def _check(x, w, d):
+    """Half a step of D's type, and FP32 accumulation: K / 32 + 32 additions (one instruction adds 32 or 64
+    products to the running sum) that lose at most a quarter step 2^-22 of the sum of magnitudes each, and the
+    scales' products."""
+    a, b = _decode(x), _decode(w)
+    want = a @ b.T
+    bound = HALF_STEP[d.dtype] * want.abs() * (1 + 2.0 ** -8) + (x.k / 32 + 32) * 2.0 ** -22 * (a.abs() @ b.abs().T)
+    if d.dtype == torch.float16:
+        bound = bound + 2.0 ** -25  # its subnormal step
+    err = (d.double() - want).abs()
+    assert (err <= bound).all(), float((err / bound.clamp(min=1e-300)).max())
+
+
+def _round_up(k, kind):
+    step = 16 if kind == "fp8" else 32
+    return -(-k // step) * step
+
+
+ROWS = [1, 2, 7, 15, 16, 17, 32, 33, 61, 64, 65, 127, 128, 129, 200, 256, 257, 300, 520]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", ROWS)
+def test_exact_rows(cuda_device, kind, m):
+    gen = torch.Generator().manual_seed(m)
+    n, k = 264, 544
+    x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+    want = _decode(x) @ _decode(w).T
+    assert torch.equal(_run(x, w, cuda_device, torch.float32).double(), want)
+    d = _run(x, w, cuda_device)
+    assert torch.equal(d, want.float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [1, 40, 130])
+@pytest.mark.parametrize("n", [1, 7, 8, 100, 127, 128, 129, 255, 257, 1000, 2052])
+def test_exact_widths(cuda_device, kind, m, n):
+    gen = torch.Generator().manual_seed(n)
+    k = 288
+    x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+    want = _decode(x) @ _decode(w).T
+    assert torch.equal(_run(x, w, cuda_device), want.float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [1, 24, 257])
+@pytest.mark.parametrize("k", [16, 32, 64, 96, 128, 144, 160, 256, 272, 512, 1040, 2880, 4096])
+def test_exact_depths(cuda_device, kind, m, k):
+    gen = torch.Generator().manual_seed(k)
+    k = _round_up(k, kind)
+    n = 140
+    x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+    want = _decode(x) @ _decode(w).T
+    # Sums of K products of at most 15 * 15 * 4: exact in FP32 below 2^24 half-units.
+    assert torch.equal(_run(x, w, cuda_device, torch.float32).double(), want)
+
+
+@pytest.mark.parametrize("dtype", list(HALF_STEP))
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n,k", [(1, 512, 4096), (5, 1000, 2880), (61, 5000, 2912), (128, 256, 8192), (200, 777, 1056),
+                                   (513, 640, 2048), (1024, 1032, 1024)])
+def test_quantised_normal(cuda_device, kind, dtype, m, n, k):
+    gen = torch.Generator().manual_seed(m + n + k)
+    x, w = _quantised_operand(kind, m, k, gen, False), _quantised_operand(kind, n, k, gen, True)
+    _check(x, w, _run(x, w, cuda_device, dtype))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", list(HALF_STEP))
+@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("n,pad,shift", [(264, 8, 0), (264, 3, 1), (96, 8, 8), (131, 0, 0)])
+def test_strided_output(cuda_device, kind, dtype, m, n, pad, shift):
+    """D inside a wider tensor; what lies beside and behind it stays as it was."""
+    gen = torch.Generator().manual_seed(n)
+    k = 160
+    x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+    full = torch.full((m + 2, n + pad + shift), -7.0, dtype=dtype, device=cuda_device)
+    _run(x, w, cuda_device, d=full[1:1 + m, shift:shift + n])
+    want = torch.full(full.shape, -7.0, dtype=dtype)
+    want[1:1 + m, shift:shift + n] = (_decode(x) @ _decode(w).T).float().to(dtype)
+    assert torch.equal(full.cpu(), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_nan_stays_in_its_row(cuda_device, kind):
+    gen = torch.Generator().manual_seed(5)
+    k, n = 256, 136
+    for m in (3, 200):
+        x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+        want = (_decode(x) @ _decode(w).T).float().to(torch.bfloat16)
+        if kind == "fp8":
+            x.data[m - 2, 7] = 0x7F
+        else:
+            bits = lowp.unpack_scale_atoms(x.atoms, m, k // (32 if kind == "mxfp4" else 16))
+            bits[m - 2, 1] = 0xFF if kind == "mxfp4" else 0x7F
+            x.atoms = lowp.pack_scale_atoms(bits)
+            if kind == "nvfp4":
+                x.scales = bits  # what .to() lays the atoms out from
+        d = _run_once(x, w, cuda_device)
+        assert torch.isnan(d[m - 2]).all()
+        keep = [i for i in range(m) if i != m - 2]
+        assert torch.equal(d[keep], want[keep])
+
+
+def _run_once(x, w, dev):
+    d = torch.empty(x.rows, w.rows, dtype=torch.bfloat16, device=dev)
+    plan = lowp.LowpLinearPlan(x.to(dev), w.to(dev), d)
+    plan.run()
+    plan.synchronize()
+    return d.cpu()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_no_rows(cuda_device, kind):
+    gen = torch.Generator().manual_seed(0)
+    w = _exact_operand(kind, 40, 64, gen, True)
+    x = {"fp8": lowp.Fp8GroupOperand, "mxfp4": lowp.Mxfp4Operand, "nvfp4": lowp.Nvfp4Operand}[kind].empty(0, 64, device="cpu")
+    assert _run(x, w, cuda_device).shape == (0, 40)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [1, 64, 260])
+def test_layer_chain(cuda_device, kind, m):
+    """Residual stream -> quantiser -> product, captured once and replayed on new tokens, beside a second
+    layer that runs on another stream at the same time."""
+    k, n = 512, 1000
+    gen = torch.Generator().manual_seed(m)
+    layers = []
+    for _ in range(2):
+        stream = torch.cuda.Stream(device=cuda_device)
+        w = _quantised_operand(kind, n, k, gen, True).to(cuda_device)
+        x = torch.empty(m, k, dtype=torch.bfloat16, device=cuda_device)
+        d = torch.empty(m, n, dtype=torch.bfloat16, device=cuda_device)
+        if kind == "fp8":
+            a = lowp.Fp8GroupOperand.empty(m, k, device=cuda_device)
+            res = torch.empty_like(x)
+            first = quantize.RmsNormFp8Plan(x, torch.ones(k, device=cuda_device), a, residual=res, residual_out=res,
+                                            stream=stream)
+        else:
+            a = (lowp.Mxfp4Operand if kind == "mxfp4" else lowp.Nvfp4Operand).empty(m, k, device=cuda_device)
+            res = None
+            first = quantize.Fp4QuantPlan(x, a, stream=stream)
+        layers.append((stream, x, res, a, w, d, first, lowp.LowpLinearPlan(a, w, d, stream=stream)))
+    torch.cuda.synchronize(cuda_device)
+    graphs = []
+    for stream, *_, first, product in layers:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            first.run()
+            product.run()
+        graphs.append(graph)
+    for step in range(3):
+        for i, (stream, x, res, *_) in enumerate(layers):
+            x.copy_(torch.randn(m, k, generator=gen).to(torch.bfloat16) * (1 + step + i))
+            if res is not None:
+                res.copy_(torch.randn(m, k, generator=gen).to(torch.bfloat16))
+        torch.cuda.synchronize(cuda_device)
+        for (stream, *_), graph in zip(layers, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize(cuda_device)
+        for stream, x, res, a, w, d, first, product in layers:
+            first.synchronize()
+            product.synchronize()
+            if kind == "fp8":  # res holds the sum now: the norm of it is what was quantised
+                y = res.double() / torch.sqrt((res.double() ** 2).mean(1, keepdim=True) + 1e-6)
+                got = _decode(a)
+                assert ((got - y).abs() <= y.abs() * 2.0 ** -4 * (1 + 2.0 ** -8)
+                        + a.scales.double().repeat_interleave(128, 1) * 2.0 ** -10).all()
+            else:
+                ref = (lowp.mxfp4_quantize if kind == "mxfp4" else lowp.nvfp4_quantize)(x.cpu())
+                assert torch.equal(a.data.cpu(), ref[0])
+            _check(a.to("cpu"), w.to("cpu"), d.cpu())
+
+
+def test_refusals_on_the_gpu(cuda_device):
+    gen = torch.Generator().manual_seed(1)
+    x, w = _exact_operand("mxfp4", 4, 64, gen, False), _exact_operand("mxfp4", 8, 64, gen, True)
+    d = torch.empty(4, 8, dtype=torch.bfloat16, device=cuda_device)
+    with pytest.raises(ValueError, match="CUDA"):
+        lowp.LowpLinearPlan(x, w.to(cuda_device), d)
+    w2 = w.to(cuda_device)
+    w2.atoms = w2.atoms[:, :0]
+    with pytest.raises(ValueError, match="scales"):
+        lowp.LowpLinearPlan(x.to(cuda_device), w2, d)
+    plan = lowp.LowpLinearPlan(x.to(cuda_device), w.to(cuda_device), d)
+    from gb300_microbench_b200 import _native as nat
+    with pytest.raises(nat.NativeCallError):
+        plan.run(-1)
+    plan.run(0)
+    assert plan.launches == 0

@@ -1,0 +1,286 @@
+"""The quantisers on the GPU: RMS norm to FP8 against the formula in 64 bits,
+the 4-bit formats against the torch definitions on the CPU bit for bit and
+against 64 bits, at odd sizes, strides, empty and non-finite rows, on other
+streams and in captured graphs."""
+import pytest
+import torch
+
+from gb300_microbench_b200 import lowp, quantize
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+U = 2.0 ** -24  # half a step of FP32, relative
+
+
+def _x(rows, cols, dtype, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp(0.5 * torch.randn(cols, generator=g)) * scale
+    return x.to(dtype)
+
+
+# ------------------------------------------------------------------ RMS norm -> FP8
+def _norm_check(x, res, weight, eps, h_got, q_got, s_got):
+    """x, res, weight on the CPU. The bounds: the sum of squares of positive terms is added in at most
+    64 + 10 + 5 steps of half a step each, the root halves that; division by the width, the added eps and
+    CUDA's rsqrtf (2 steps) and the two products of y add 2 + 4 + 2 half steps; a scale's division one more."""
+    h = x if res is None else (x.float() + res.float()).to(x.dtype)
+    if h_got is not None:
+        assert torch.equal(h_got, h)
+    f = h.double()
+    cols = f.shape[1]
+    y = f / torch.sqrt((f * f).sum(1, keepdim=True) / cols + eps) * weight.double()
+    groups = -(-cols // 128)
+    amax = torch.nn.functional.pad(y, (0, groups * 128 - cols)).view(-1, groups, 128).abs().amax(2)
+    s = torch.where(amax > 0, amax / 448, 1.0)
+    rel = (79 / 2 + 8 + 1) * U
+    assert ((s_got.double() - s).abs() <= rel * s).all()
+    # q is e4m3(y / s): half a step of E4M3 around a quotient that is off by what y and s are.
+    want = y / s.repeat_interleave(128, 1)[:, :cols]
+    half = torch.maximum(want.abs() * 2.0 ** -4, torch.full_like(want, 2.0 ** -10))
+    err = (q_got.double() - want).abs()
+    assert (err <= half * (1 + 2.0 ** -10) + 2 * rel * want.abs()).all(), float((err / half).max())
+
+
+def _norm(x, weight, dev, res=None, eps=1e-6, store=True, stream=None):
+    out = lowp.Fp8GroupOperand.empty(*x.shape, device=dev)
+    xd, rd = x.to(dev), None if res is None else res.to(dev)
+    ro = torch.empty_like(xd) if store else None
+    plan = quantize.RmsNormFp8Plan(xd, weight.to(dev), out, residual=rd, residual_out=ro, eps=eps, stream=stream)
+    plan.run()
+    plan.synchronize()
+    assert plan.launches == (1 if x.shape[0] else 0)
+    plan.close()
+    return None if ro is None else ro.cpu(), out.values.float().cpu(), out.scales.cpu()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 8), (3, 7), (2, 128), (5, 129), (4, 255), (1, 4096), (33, 2880),
+                                       (7, 2900), (3, 8192), (2, 12288), (1, 32768), (2, 32776), (1, 65536),
+                                       (1, 65535), (300, 257)])
+def test_norm_sizes(cuda_device, dtype, rows, cols):
+    x, res = _x(rows, cols, dtype), _x(rows, cols, dtype, seed=1, scale=3.0)
+    w = (1 + 0.1 * torch.randn(cols, generator=torch.Generator().manual_seed(2))).to(dtype)
+    _norm_check(x, res, w, 1e-6, *_norm(x, w, cuda_device, res))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_without_residual_and_fp32_weight(cuda_device, dtype):
+    x, w = _x(9, 520, dtype), torch.linspace(-2, 2, 520)
+    _, q, s = _norm(x, w, cuda_device, store=False, eps=0.0)
+    _norm_check(x, None, w, 0.0, None, q, s)
+
+
+@pytest.mark.parametrize("pad,shift", [(8, 0), (1, 0), (3, 1), (8, 4)])
+def test_norm_strides(cuda_device, pad, shift):
+    """Rows inside wider tensors, aligned and not; what lies beside them stays."""
+    rows, cols = 6, 264
+    full = _x(rows, cols + pad + shift, torch.bfloat16, seed=4).to(cuda_device)
+    res_full = _x(rows, cols + pad + shift, torch.bfloat16, seed=5).to(cuda_device)
+    before = res_full.clone()
+    x, res = full[:, shift:shift + cols], res_full[:, shift:shift + cols]
+    w = torch.ones(cols, dtype=torch.bfloat16, device=cuda_device)
+    out = lowp.Fp8GroupOperand.empty(rows, cols, device=cuda_device)
+    x0, r0 = x.cpu().clone(), res.cpu().clone()
+    plan = quantize.RmsNormFp8Plan(x, w, out, residual=res, residual_out=res)  # in place
+    plan.run()
+    plan.synchronize()
+    _norm_check(x0, r0, w.cpu(), 1e-6, res.cpu().clone(), out.values.float().cpu(), out.scales.cpu())
+    side = torch.ones(cols + pad + shift, dtype=torch.bool)
+    side[shift:shift + cols] = False
+    assert torch.equal(res_full[:, side.to(cuda_device)], before[:, side.to(cuda_device)])
+
+
+def test_norm_zero_and_non_finite_rows(cuda_device):
+    x = _x(5, 300, torch.float32)
+    x[1] = 0
+    x[2, 130] = float("nan")
+    x[3, 5] = float("inf")
+    w = torch.ones(300)
+    _, q, s = _norm(x, w, cuda_device, store=False)
+    for r in (0, 4):
+        _norm_check(x[r:r + 1], None, w, 1e-6, None, q[r:r + 1], s[r:r + 1])
+    assert (q[1] == 0).all() and (s[1] == 1).all()
+    assert torch.isnan(q[2]).all() and torch.isnan(s[2]).all()
+    assert torch.isnan(q[3, 5]) and torch.isnan(s[3, 0])
+
+
+def test_norm_no_rows(cuda_device):
+    x = torch.empty(0, 64, dtype=torch.bfloat16)
+    h, q, s = _norm(x, torch.ones(64), cuda_device)
+    assert h.shape == (0, 64) and q.shape == (0, 64) and s.shape == (0, 1)
+
+
+def test_norm_rows_of_few_steps_are_exact(cuda_device):
+    """One non-zero element a row: y = sqrt(cols) * sign * w, q = +-448."""
+    x = torch.zeros(64, 64, dtype=torch.float16)
+    x.fill_diagonal_(-3.0)
+    _, q, s = _norm(x, torch.ones(64), cuda_device, store=False, eps=0.0)
+    assert torch.equal(q, torch.eye(64) * -448)
+    assert ((s.double() - 8 / 448).abs() <= 10 * U * 8 / 448).all()
+
+
+# ------------------------------------------------------------------ 4-bit formats
+def _operand(fmt, rows, k, dev, scale):
+    if fmt == "mxfp4":
+        return lowp.Mxfp4Operand.empty(rows, k, device=dev)
+    return lowp.Nvfp4Operand.empty(rows, k, device=dev, tensor_scale=scale)
+
+
+def _fp4(fmt, x, dev, scale=None, values=True, stream=None):
+    op = _operand(fmt, *x.shape, dev, scale)
+    op.data.fill_(0xAA)
+    op.atoms.fill_(0xAA)
+    xd = x.to(dev)
+    v = torch.full_like(xd, float("nan")) if values else None
+    plan = quantize.Fp4QuantPlan(xd, op, values=v, stream=stream)
+    plan.run()
+    plan.synchronize()
+    plan.close()
+    return op.to("cpu"), None if v is None else v.cpu()
+
+
+def _fp4_reference(fmt, x, scale=None):
+    if fmt == "mxfp4":
+        packed, bits = lowp.mxfp4_quantize(x)
+        return packed, bits, None, lowp.mxfp4_dequantize(packed, bits)
+    packed, bits, g = lowp.nvfp4_quantize(x, scale)
+    return packed, bits, g, lowp.nvfp4_dequantize(packed, bits, g)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt,scale", [("mxfp4", None), ("nvfp4", None), ("nvfp4", 0.003)])
+@pytest.mark.parametrize("rows,k", [(1, 32), (1, 64), (2, 96), (127, 160), (129, 32), (77, 4096), (300, 288), (5, 2880)])
+def test_fp4_equals_definition(cuda_device, fmt, scale, dtype, rows, k):
+    x = _x(rows, k, dtype, seed=rows)
+    packed, bits, g, deq = _fp4_reference(fmt, x, scale)
+    op, v = _fp4(fmt, x, cuda_device, scale)
+    assert torch.equal(op.atoms, lowp.pack_scale_atoms(bits))  # padding rows and columns zero
+    assert torch.equal(op.data, packed)
+    assert torch.equal(v, deq.to(dtype))
+    if fmt == "nvfp4" and scale is None:
+        assert float(op.tensor_scale_out) == float(torch.tensor(g, dtype=torch.float32))
+    assert torch.equal(op.dequantize(), deq)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_fp4_against_64_bits(cuda_device, fmt):
+    """Each value is the nearest of the block's grid: half a step around a quotient whose divisor and
+    result were rounded once each (nvfp4; mxfp4 divides exactly)."""
+    x = _x(130, 512, torch.float32, seed=9)
+    op, v = _fp4(fmt, x, cuda_device, values=True)
+    block, bits = (32, None) if fmt == "mxfp4" else (16, None)
+    width = 512 // block
+    bits = lowp.unpack_scale_atoms(op.atoms, 130, width)
+    unit = lowp.mxfp4_scale_values(bits).double() if fmt == "mxfp4" else \
+        bits.view(torch.float8_e4m3fn).double() * float(op.tensor_scale_out)
+    unit = unit.repeat_interleave(block, 1)
+    y = (x.double() / unit).abs()
+    # The block's scale may leave amax / scale above 6 by its own rounding (mxfp4: below 8); cut there.
+    q = (v.double() / unit).abs()
+    step = torch.where(y < 2, 0.5, torch.where(y < 4, 1.0, 2.0))
+    slack = 0.0 if fmt == "mxfp4" else 4 * U
+    ok = ((q - y).abs() <= step / 2 + slack * y) | ((y > 6) & ((q - 6).abs() <= slack * 6))
+    assert ok.all()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("magnitude", [1e-42, 1e-36, 1e-20, 1e20, 1e37])
+def test_fp4_range(cuda_device, fmt, magnitude):
+    x = _x(40, 128, torch.float32, seed=11)
+    x = x / x.abs().max() * magnitude
+    x[3, :64] = 0
+    x[4] = 0
+    packed, bits, g, deq = _fp4_reference(fmt, x)
+    op, v = _fp4(fmt, x, cuda_device)
+    assert torch.equal(op.atoms, lowp.pack_scale_atoms(bits))
+    assert torch.equal(op.data, packed) and torch.equal(v, deq)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_fp4_non_finite(cuda_device, fmt):
+    x = _x(4, 96, torch.float32, seed=12)
+    x[0, 3], x[1, 40], x[2, 95] = float("nan"), float("inf"), float("-inf")
+    packed, bits, g, deq = _fp4_reference(fmt, x, 0.01)
+    op, v = _fp4(fmt, x, cuda_device, scale=0.01 if fmt == "nvfp4" else None)
+    assert torch.equal(op.atoms, lowp.pack_scale_atoms(bits))
+    assert torch.equal(op.data, packed)
+    assert torch.equal(torch.isnan(v), torch.isnan(deq)) and torch.equal(v.nan_to_num(), deq.nan_to_num())
+    assert not torch.isnan(v[3]).any()
+
+
+def test_fp4_borders(cuda_device):
+    """Quotients on and one step beside every border of the grid."""
+    mids = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0])
+    rows = []
+    for scale in (1.0, 3.0, 0.7, 1.3e-5, 7.7e4):
+        for direction in (0.0, 1e9, -1e9):
+            m = mids * scale
+            m = torch.nextafter(m, torch.full_like(m, direction)) if direction else m
+            m[-1] = 6 * scale
+            rows.append(torch.cat((m, -m)).repeat(4))
+    x = torch.stack(rows)
+    for fmt, scale in (("mxfp4", None), ("nvfp4", None), ("nvfp4", 1e-3), ("nvfp4", 0.37)):
+        packed, bits, _, deq = _fp4_reference(fmt, x, scale)
+        op, v = _fp4(fmt, x, cuda_device, scale)
+        assert torch.equal(op.atoms, lowp.pack_scale_atoms(bits))
+        assert torch.equal(op.data, packed) and torch.equal(v, deq)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("shift", [0, 1, 8])
+def test_fp4_strides_and_in_place(cuda_device, fmt, shift):
+    full = _x(20, 96 + 16, torch.bfloat16, seed=13).to(cuda_device)
+    keep = full.clone()
+    x = full[:, shift:shift + 96]
+    packed, bits, _, deq = _fp4_reference(fmt, x.cpu(), 0.01)
+    op = _operand(fmt, 20, 96, cuda_device, 0.01)
+    plan = quantize.Fp4QuantPlan(x, op, values=x)
+    plan.run()
+    plan.synchronize()
+    assert torch.equal(op.data.cpu(), packed) and torch.equal(op.atoms.cpu(), lowp.pack_scale_atoms(bits))
+    assert torch.equal(x.cpu(), deq.to(torch.bfloat16))
+    assert torch.equal(full[:, :shift], keep[:, :shift]) and torch.equal(full[:, shift + 96:], keep[:, shift + 96:])
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_fp4_no_rows(cuda_device, fmt):
+    op, v = _fp4(fmt, torch.empty(0, 64, dtype=torch.bfloat16), cuda_device)
+    assert op.data.shape == (0, 32) and v.shape == (0, 64)
+
+
+def test_division_is_exact_for_many_quotients(cuda_device):
+    """The quotient by residual against torch's division: NVFP4 with tensor scale 1 and block maxima that
+    make the block scale 1, so values are q(x / g) for many g and random x; compared through the codes."""
+    g = torch.Generator().manual_seed(21)
+    x = torch.rand(4096, 512, generator=g) * 6
+    scale = torch.exp(3 * torch.randn(8, generator=g)).tolist()
+    for s in scale:
+        packed, bits, _, _ = _fp4_reference("nvfp4", x, s)
+        op, _ = _fp4("nvfp4", x, cuda_device, s, values=False)
+        assert torch.equal(op.atoms, lowp.pack_scale_atoms(bits)) and torch.equal(op.data, packed)
+
+
+# ------------------------------------------------------------------ streams and graphs
+def test_other_stream_and_graph(cuda_device):
+    """Plans on a stream of their own, captured and replayed on new data."""
+    stream = torch.cuda.Stream(device=cuda_device)
+    x = _x(17, 320, torch.bfloat16).to(cuda_device)
+    w = torch.ones(320, device=cuda_device)
+    fp8 = lowp.Fp8GroupOperand.empty(17, 320, device=cuda_device)
+    nv = lowp.Nvfp4Operand.empty(17, 320, device=cuda_device)
+    stream.wait_stream(torch.cuda.current_stream(cuda_device))
+    plans = [quantize.RmsNormFp8Plan(x, w, fp8, stream=stream), quantize.Fp4QuantPlan(x, nv, stream=stream)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for p in plans:
+            p.run()
+    for seed in (30, 31):
+        new = _x(17, 320, torch.bfloat16, seed=seed, scale=1 + seed)
+        x.copy_(new.to(cuda_device))
+        graph.replay()
+        torch.cuda.synchronize(cuda_device)
+        _norm_check(new, None, w.cpu(), 1e-6, None, fp8.values.float().cpu(), fp8.scales.cpu())
+        packed, bits, g, _ = _fp4_reference("nvfp4", new)
+        assert torch.equal(nv.data.cpu(), packed) and torch.equal(nv.atoms.cpu(), lowp.pack_scale_atoms(bits))
+        assert float(nv.tensor_scale_out) == float(torch.tensor(g, dtype=torch.float32))
