@@ -1,98 +1,373 @@
 // The product of a quantised linear layer, D (M x N) = dequant(A) * dequant(B)^T,
 // for any number of rows (bb_linear_*): NVFP4, MXFP4, and FP8 with activations
 // scaled per row and 128 K elements and weights per 128 x 128 block.
-#include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
-#include <atomic>
+//
+// Many rows run the 256 x 256 (128 x 256) tile kernel of gemm_lowp.cuh. Few
+// rows run the kernel below, whose work is to read the weights once.
 #include <new>
 
-#include "common.cuh"
-#include "ptx.cuh"
+#include "gemm_lowp.cuh"
 
 namespace bb {
-extern std::atomic<int64_t> g_kernel_launches;
-
 namespace linear {
 
-struct SimpleParams {
-  int32_t m, n, k, atoms_k;
-  const uint8_t* a;
-  const uint8_t* b;
-  const uint8_t* sfa;
-  const uint8_t* sfb;
-  int64_t sfa_ld, ldd;
-  float scale_a, scale_b;
-  const float* scale_a_dev;
-  const float* scale_b_dev;
-  void* d;
-  int32_t d_dtype;
+using namespace lowp;
+
+// ---------------------------------------------------------------- few rows
+// D^T = W * X^T: the weights' rows are the tensor core's M = 128 (all of them
+// useful), the TN tokens its N (16 upwards), so one token costs the same weight
+// stream as sixteen and no arithmetic unit decodes a weight. A CTA streams
+// 128 weight rows over one share of K; the `splits` CTAs of a cluster share K
+// and add their FP32 partial sums over distributed shared memory, in rank
+// order (the result does not depend on timing).
+//
+// FP8: the K blocks' FP32 scales are applied as in the tile kernel, each
+// block accumulated alone in one of kBufs TMEM buffers and promoted by the
+// epilogue warps: acc[c] += part[c] * sa[token c][kb] * sb[kb].
+//
+// Bound by DRAM at one CTA pair per SM: two CTAs of up to 113 KiB share an SM
+// (TN <= 128), so about 200 KiB of weights per SM are in flight.
+template <int kKind, int kTN>
+struct FewCfg {
+  static constexpr int TN = kTN;
+  static constexpr bool FP4 = is_fp4(kKind);
+  static constexpr int CTAS_PER_SM = TN <= 128 ? 2 : 1;
+  static constexpr int EPI_W = TN <= 32 ? 4 : 8;  // epilogue warps: lane quarters x column halves
+  static constexpr int THREADS = 64 + 32 * EPI_W;
+  static constexpr int COLS = TN * 4 / EPI_W;     // accumulator columns per epilogue thread
+  static constexpr int K_PER_STAGE = FP4 ? 256 : 128;
+  static constexpr int MMAS = 4;
+  static constexpr int ATOMS = kKind == kNvfp4 ? 4 : kKind == kMxfp4 ? 2 : 0;
+  static constexpr int X_BLOCKS = TN > 128 ? 2 : 1;  // 128-row scale blocks of the tokens
+  static constexpr int W_BYTES = 128 * ROW_BYTES;
+  static constexpr int X_BYTES = TN * ROW_BYTES;
+  static constexpr int SFW_BYTES = ATOMS * SF_ATOM;
+  static constexpr int SFX_BYTES = X_BLOCKS * ATOMS * SF_ATOM;
+  static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + SFW_BYTES + SFX_BYTES;
+  static constexpr int SCALE_BYTES = FP4 ? 0 : EPI_W * COLS * 4;  // FP8: a K block's scales, per epilogue warp
+  static constexpr int TAIL_BYTES = SCALE_BYTES + BAR_BYTES;
+  static constexpr int LIMIT = CTAS_PER_SM == 2 ? 115712 : SMEM_LIMIT;
+  static constexpr int STAGES_FIT = (LIMIT - 1024 - TAIL_BYTES) / STAGE_BYTES;
+  static constexpr int STAGES = STAGES_FIT < 8 ? STAGES_FIT : 8;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TAIL_BYTES;
+  // FP8: partial buffers. FP4: one accumulator, then the scale columns.
+  static constexpr int BUFS = FP4 ? 1 : TN <= 32 ? 4 : 2;
+  static constexpr int SF_COL = TN;
+  static constexpr int SF_COLS = ATOMS * 4 * (1 + X_BLOCKS);
+  static constexpr int COLS_USED = FP4 ? TN + SF_COLS : BUFS * TN;
+  static constexpr int TMEM = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
+  static_assert(TMEM * CTAS_PER_SM <= 512, "TMEM of the CTAs that share an SM");
+  static_assert(STAGES >= 3 && SMEM_BYTES <= LIMIT, "shared memory");
+  static_assert(TN * 128 * 4 <= STAGES * STAGE_BYTES, "partial sums fit the ring");
+  static_assert((2 * STAGES + 2 * BUFS + 3) * 8 <= BAR_BYTES, "barrier area");
+  static_assert(BUFS < STAGES, "a stage's barrier tells the epilogue of its block");
 };
 
-__device__ __forceinline__ float e2m1(uint32_t code) {
-  const uint32_t e = (code >> 1) & 3u, m = code & 1u;
-  const float mag = e == 0 ? 0.5f * m : __uint_as_float((126u + e) << 23 | m << 22);
-  return (code & 8u) ? -mag : mag;
-}
-__device__ __forceinline__ float e4m3(uint8_t b) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
-}
-__device__ __forceinline__ float e8m0(uint8_t b) {
-  return b == 255 ? __uint_as_float(0x7fc00000u) : b ? __uint_as_float(static_cast<uint32_t>(b) << 23) : 0x1p-127f;
-}
-__device__ __forceinline__ uint8_t atom_byte(const uint8_t* atoms, int row, int atoms_k, int j) {
-  const int r = row % 128;
-  return atoms[(static_cast<int64_t>(row / 128) * atoms_k + j / 4) * 512 + (r % 32) * 16 + (r / 32) * 4 + j % 4];
+struct FewParams {
+  int32_t m, n;
+  int32_t k_stages, splits, tiles_n;
+  int32_t kb;          // FP8: K blocks
+  const float* sfa;    // FP8: [kb][sfa_ld]
+  const float* sfb;    // FP8: [n blocks][kb]
+  int64_t sfa_ld, ldd;
+  float scale;
+  const float* scale_dev[2];
+  void* d;
+  int32_t d_dtype;
+  int* status;
+};
+
+__device__ __forceinline__ void store_one(void* d, int dtype, int64_t at, float v) {
+  if (dtype == BB_DTYPE_BF16) static_cast<__nv_bfloat16*>(d)[at] = __float2bfloat16_rn(v);
+  else if (dtype == BB_DTYPE_F16) static_cast<__half*>(d)[at] = __float2half_rn(v);
+  else static_cast<float*>(d)[at] = v;
 }
 
-// 64 x 64 outputs per block of 256 threads, 32 K elements at a time dequantised into shared memory.
-template <int kKind>
-__global__ void __launch_bounds__(256) simple_linear_kernel(const SimpleParams p) {
-  __shared__ float sa[32][65], sb[32][65];
-  const int tiles_n = (p.n + 63) / 64;
-  const int m0 = blockIdx.x / tiles_n * 64, n0 = blockIdx.x % tiles_n * 64;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  const int kb = (p.k + 127) / 128;
-  auto value = [&](bool weights, int row, int k) -> float {
-    if (row >= (weights ? p.n : p.m) || k >= p.k) return 0.f;
-    const uint8_t* v = weights ? p.b : p.a;
-    const uint8_t* s = weights ? p.sfb : p.sfa;
-    if constexpr (kKind == BB_LOWP_FP8_GROUP128) {
-      const float* f = reinterpret_cast<const float*>(s);
-      const float scale = weights ? f[static_cast<int64_t>(row / 128) * kb + k / 128] : f[(k / 128) * p.sfa_ld + row];
-      return e4m3(v[static_cast<int64_t>(row) * p.k + k]) * scale;
-    } else {
-      const uint8_t byte = v[static_cast<int64_t>(row) * (p.k / 2) + k / 2];
-      const float q = e2m1(k % 2 ? byte >> 4 : byte & 15u);
-      if constexpr (kKind == BB_LOWP_MXFP4) return q * e8m0(atom_byte(s, row, p.atoms_k, k / 32));
-      return q * e4m3(atom_byte(s, row, p.atoms_k, k / 16));
-    }
-  };
-  for (int k0 = 0; k0 < p.k; k0 += 32) {
-    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-      sa[i % 32][i / 32] = value(false, m0 + i / 32, k0 + i % 32);
-      sb[i % 32][i / 32] = value(true, n0 + i / 32, k0 + i % 32);
-    }
-    __syncthreads();
-    for (int k = 0; k < 32; ++k)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty + 16 * i], sb[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
+// N columns of this warp's 32 TMEM lanes.
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t* r) {
+  if constexpr (N >= 32) {
+#pragma unroll
+    for (int c = 0; c < N / 32; ++c) tmem_ld_32x32b_x32(taddr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
+  } else {
+    static_assert(N == 16, "16 or a multiple of 32");
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
   }
-  const float g = (p.scale_a_dev ? *p.scale_a_dev : p.scale_a) * (p.scale_b_dev ? *p.scale_b_dev : p.scale_b);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m >= p.m || n >= p.n) continue;
-      const int64_t at = m * p.ldd + n;
-      const float v = acc[i][j] * g;
-      if (p.d_dtype == BB_DTYPE_BF16) static_cast<__nv_bfloat16*>(p.d)[at] = __float2bfloat16_rn(v);
-      else if (p.d_dtype == BB_DTYPE_F16) static_cast<__half*>(p.d)[at] = __float2half_rn(v);
-      else static_cast<float*>(p.d)[at] = v;
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+template <int kKind, int kTN>
+__global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN>::CTAS_PER_SM)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                    const __grid_constant__ CUtensorMap tm_sfw, const __grid_constant__ CUtensorMap tm_sfx,
+                    const FewParams p) {
+  using C = FewCfg<kKind, kTN>;
+  constexpr int STAGES = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem_w = smem;
+  uint8_t* smem_x = smem_w + STAGES * C::W_BYTES;
+  uint8_t* smem_sfw = smem_x + STAGES * C::X_BYTES;
+  uint8_t* smem_sfx = smem_sfw + STAGES * C::SFW_BYTES;
+  float* smem_scale = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES + C::SCALE_BYTES);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + STAGES;
+  uint64_t* acc_empty = bars + 2 * STAGES;  // [BUFS], FP8
+  uint64_t* done = acc_empty + C::BUFS;     // every MMA of this CTA has finished
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit = blockIdx.x / p.splits;  // (token tile, weight row block)
+  const int m0 = unit / p.tiles_n * C::TN, n_blk = unit % p.tiles_n;
+  const int ks0 = static_cast<int>(static_cast<int64_t>(p.k_stages) * rank / p.splits);
+  const int ks1 = static_cast<int>(static_cast<int64_t>(p.k_stages) * (rank + 1) / p.splits);
+
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_x);
+    if constexpr (C::FP4) {
+      prefetch_tmap(&tm_sfw);
+      prefetch_tmap(&tm_sfx);
     }
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    for (int b = 0; b < C::BUFS; ++b) mbar_init(smem_u32(&acc_empty[b]), C::EPI_W);
+    mbar_init(smem_u32(done), 1);
+    fence_mbarrier_init_cluster();
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(smem_u32(tmem_slot), C::TMEM);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  float scale = p.scale;
+  float* red = reinterpret_cast<float*>(smem);  // [TN][128] partial sums, over the ring once it is idle
+  const int q = warp & 3, half = (warp - 2) / 4;
+  const int row = q * 32 + lane;       // weight row within the block (epilogue)
+  const int col0 = half * C::COLS;     // first token of this thread (epilogue)
+  const int n = n_blk * 128 + row;
+  auto put = [&](int c, float v) {
+    const int m = m0 + c;
+    if (m < p.m && n < p.n) store_one(p.d, p.d_dtype, m * p.ldd + n, v * scale);
+  };
+
+  if (warp == 0) {
+    bool ok = true;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int ks = ks0; ks < ks1; ++ks) {
+      if (!bb_wait_warp(smem_u32(&empty[stage]), phase ^ 1u, p.status, kDevTimeoutProducer)) {
+        ok = false;
+        break;
+      }
+      if (elect_one()) {
+        const uint32_t fb = smem_u32(&full[stage]);
+        mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
+        tma_load_2d(smem_u32(smem_w + stage * C::W_BYTES), &tm_w, fb, ks * ROW_BYTES, n_blk * 128);
+        tma_load_2d(smem_u32(smem_x + stage * C::X_BYTES), &tm_x, fb, ks * ROW_BYTES, m0);
+        if constexpr (C::FP4) {
+          tma_load_2d(smem_u32(smem_sfw + stage * C::SFW_BYTES), &tm_sfw, fb, ks * 64 * C::ATOMS, n_blk);
+          tma_load_2d(smem_u32(smem_sfx + stage * C::SFX_BYTES), &tm_sfx, fb, ks * 64 * C::ATOMS, m0 / 128);
+        }
+      }
+      __syncwarp();
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (ok) {
+      // Tail: until the MMAs released every stage, so no commit is on its way to a CTA that left.
+      for (int i = 0; i < STAGES; ++i) {
+        if (!bb_wait_warp(smem_u32(&empty[stage]), phase ^ 1u, p.status, kDevTimeoutProducer)) break;
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    } else if (lane == 0) {
+      bounded_sleep_ns(2000000);  // aborted: let copies already issued land
+    }
+  } else if (warp == 1) {
+    int stage = 0;
+    uint32_t phase = 0, it = 0;
+    const uint64_t w_desc0 = sw128_kmajor_desc(smem_u32(smem_w)), x_desc0 = sw128_kmajor_desc(smem_u32(smem_x));
+    const uint64_t sfw_desc0 = sf_atom_desc(smem_u32(smem_sfw)), sfx_desc0 = sf_atom_desc(smem_u32(smem_sfx));
+    for (int ks = ks0; ks < ks1; ++ks, ++it) {
+      if (!bb_wait_warp<false, false>(smem_u32(&full[stage]), phase, p.status, kDevTimeoutMma)) break;
+      uint32_t d_tmem = tmem;
+      if constexpr (!C::FP4) {
+        const uint32_t buf = it % C::BUFS;
+        if (!bb_wait_warp<false, false>(smem_u32(&acc_empty[buf]), ((it / C::BUFS) & 1u) ^ 1u, p.status,
+                                        kDevTimeoutMma))
+          break;
+        d_tmem += buf * C::TN;
+      }
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t w_desc = w_desc0 + static_cast<uint64_t>(stage) * (C::W_BYTES >> 4);
+        const uint64_t x_desc = x_desc0 + static_cast<uint64_t>(stage) * (C::X_BYTES >> 4);
+        if constexpr (C::FP4) {
+          const uint64_t sfw = sfw_desc0 + static_cast<uint64_t>(stage) * (C::SFW_BYTES >> 4);
+          const uint64_t sfx = sfx_desc0 + static_cast<uint64_t>(stage) * (C::SFX_BYTES >> 4);
+          constexpr int per_atom = C::MMAS / C::ATOMS;  // instructions that share an atom
+#pragma unroll
+          for (int g = 0; g < C::MMAS; ++g) {
+            const int a = g / per_atom;
+            const uint32_t t_w = tmem + C::SF_COL + 4 * a;
+            const uint32_t t_x = tmem + C::SF_COL + 4 * C::ATOMS + 4 * C::X_BLOCKS * a;
+            if (g % per_atom == 0) {
+              tmem_cp_desc<1>(t_w, sfw + a * (SF_ATOM >> 4));
+#pragma unroll
+              for (int b = 0; b < C::X_BLOCKS; ++b)
+                tmem_cp_desc<1>(t_x + 4 * b, sfx + (b * C::ATOMS + a) * (SF_ATOM >> 4));
+            }
+            const uint32_t acc = (it | g) != 0 ? 1u : 0u;
+            // A 64-token tile may begin in the middle of a 128-row scale block: 32 rows a column.
+            const uint32_t t_xs = t_x + static_cast<uint32_t>(m0 % 128) / 32;
+            if constexpr (kKind == kNvfp4)
+              mma_nvf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_nvf4(128, C::TN), t_w, t_xs, acc);
+            else
+              mma_mxf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_mxf4(128, C::TN, 2 * (g % 2)), t_w, t_xs, acc);
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < C::MMAS; ++g)
+            mma_f8<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_f8(128, C::TN), g != 0 ? 1u : 0u);
+        }
+        umma_commit<1>(smem_u32(&empty[stage]));
+      }
+      __syncwarp();
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    // Tracks every MMA issued: the accumulator is complete, the ring idle.
+    if (elect_one()) umma_commit<1>(smem_u32(done));
+    __syncwarp();
+    bb_wait_warp(smem_u32(done), 0, p.status, kDevTimeoutMma, /*honor_abort=*/false);
+  } else {
+    if (p.scale_dev[0]) scale *= *p.scale_dev[0];
+    if (p.scale_dev[1]) scale *= *p.scale_dev[1];
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + col0;
+    float acc[C::COLS];
+    bool ok = true;
+    if constexpr (C::FP4) {
+      ok = bb_wait_warp(smem_u32(done), 0, p.status, kDevTimeoutEpilogue);
+      tc_fence_after();
+      if (ok) {
+        tmem_ld_cols<C::COLS>(taddr, reinterpret_cast<uint32_t*>(acc));
+        tmem_ld_wait();
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < C::COLS; ++c) acc[c] = 0.f;
+      float* my_scale = smem_scale + (warp - 2) * C::COLS;  // this warp's token scales of the current K block
+      constexpr int kPer = (C::COLS + 31) / 32;
+      float next[kPer], next_b = 0.f;
+      auto load = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int c = lane + 32 * j;
+          next[j] = c < C::COLS && m0 + col0 + c < p.m ? __ldg(p.sfa + kb * p.sfa_ld + m0 + col0 + c) : 0.f;
+        }
+        next_b = __ldg(p.sfb + static_cast<int64_t>(n_blk) * p.kb + kb);
+      };
+      load(ks0);
+      for (int ks = ks0; ks < ks1; ++ks) {
+        const uint32_t it = ks - ks0, buf = it % C::BUFS;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (lane + 32 * j < C::COLS) my_scale[lane + 32 * j] = next[j] * next_b;
+        __syncwarp();
+        if (ks + 1 < ks1) load(ks + 1);
+        // The commit that releases the operand stage also says that the K
+        // block's partial is complete; the MMA warp runs at most BUFS < STAGES
+        // blocks ahead, so the parity cannot be overtaken.
+        if (!bb_wait_warp<false, false>(smem_u32(&empty[it % STAGES]), (it / STAGES) & 1u, p.status,
+                                        kDevTimeoutEpilogue)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        constexpr int kChunk = C::COLS < 32 ? C::COLS : 32;
+#pragma unroll
+        for (int c0 = 0; c0 < C::COLS; c0 += kChunk) {
+          uint32_t r[kChunk];
+          tmem_ld_cols<kChunk>(taddr + buf * C::TN + c0, r);
+          tmem_ld_wait();
+          if (c0 + kChunk == C::COLS) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&acc_empty[buf]));
+          }
+#pragma unroll
+          for (int c = 0; c < kChunk; c += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(my_scale + c0 + c);
+            acc[c0 + c] = fmaf(__uint_as_float(r[c]), s.x, acc[c0 + c]);
+            acc[c0 + c + 1] = fmaf(__uint_as_float(r[c + 1]), s.y, acc[c0 + c + 1]);
+            acc[c0 + c + 2] = fmaf(__uint_as_float(r[c + 2]), s.z, acc[c0 + c + 2]);
+            acc[c0 + c + 3] = fmaf(__uint_as_float(r[c + 3]), s.w, acc[c0 + c + 3]);
+          }
+        }
+      }
+      if (p.splits > 1) ok = ok && bb_wait_warp(smem_u32(done), 0, p.status, kDevTimeoutEpilogue);
+    }
+    if (ok) {
+      if (p.splits == 1) {
+#pragma unroll
+        for (int c = 0; c < C::COLS; ++c) put(col0 + c, acc[c]);
+      } else {
+        // The ring is idle (`done`): no copy is in flight and every MMA has read its operands.
+#pragma unroll
+        for (int c = 0; c < C::COLS; ++c)
+          if (m0 + col0 + c < p.m) red[(col0 + c) * 128 + row] = acc[c];
+      }
+    }
+  }
+  if (p.splits > 1) {
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 2) {
+      // Rank r adds the tokens r, r + splits, ... of all ranks' partial sums.
+      const int tokens = min(C::TN, p.m - m0);
+      const uint32_t base = smem_u32(red) + row * 4;
+      for (int c = rank + half * p.splits; c < tokens; c += p.splits * (C::EPI_W / 4)) {
+        float v = 0.f;
+        for (int r = 0; r < p.splits; ++r) v += ld_cluster_f32(mapa_shared(base + c * 512, r));
+        put(c, v);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while another reads its partial sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, C::TMEM);
+  }
 }
 
 }  // namespace linear
@@ -104,10 +379,184 @@ using namespace bb::linear;
 struct bb_linear_plan {
   int kind = 0, device = 0;
   cudaStream_t stream = nullptr;
-  SimpleParams params{};
+  bool few = false;
+  int tn = 0;      // few rows: tokens of a tile
+  int cg = 1;      // tiles: CTAs of a tile
+  bool direct = false;
+  CUtensorMap tm_a{}, tm_b{}, tm_sfa{}, tm_sfb{}, tm_d{};
+  Params tile{};
+  FewParams fp{};
+  int grid = 0;
   int* status_dev = nullptr;
   int64_t launches = 0;
 };
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+// Attributes are per device: one call per kernel and device.
+template <typename K>
+int allow_smem(K kernel, int bytes, int device, bool (&done)[kMaxDevices]) {
+  if (device < kMaxDevices && done[device]) return BB_OK;
+  BB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (device < kMaxDevices) done[device] = true;
+  return BB_OK;
+}
+
+cudaLaunchConfig_t config(int grid, int threads, int smem, int cluster, cudaStream_t stream, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+template <int kKind, int kTN>
+int launch_few(const bb_linear_plan& pl) {
+  using C = FewCfg<kKind, kTN>;
+  static bool done[kMaxDevices] = {};
+  auto kernel = few_rows_kernel<kKind, kTN>;
+  int rc = allow_smem(kernel, C::SMEM_BYTES, pl.device, done);
+  if (rc != BB_OK) return rc;
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = config(pl.grid, C::THREADS, C::SMEM_BYTES, pl.fp.splits, pl.stream, attr);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, pl.tm_b, pl.tm_a, pl.tm_sfb, pl.tm_sfa, pl.fp),
+                    "launch few_rows_kernel");
+}
+
+template <int kKind>
+int launch_few_kind(const bb_linear_plan& pl) {
+  switch (pl.tn) {
+    case 16: return launch_few<kKind, 16>(pl);
+    case 32: return launch_few<kKind, 32>(pl);
+    case 64: return launch_few<kKind, 64>(pl);
+    case 128: return launch_few<kKind, 128>(pl);
+    default: return launch_few<kKind, 256>(pl);
+  }
+}
+
+template <int kKind, int kCG, bool kDirect>
+int launch_tile(const bb_linear_plan& pl) {
+  using C = Cfg<kKind, kCG>;
+  static bool done[kMaxDevices] = {};
+  auto kernel = bb_lowp_gemm_kernel<kKind, kCG, true, kDirect>;
+  if (pl.device >= kMaxDevices || !done[pl.device]) {
+    if constexpr (C::kRegSplit) {
+      // setmaxnreg.inc waits until the block's register pool can serve it;
+      // refuse to launch a build whose pool is smaller than the split needs.
+      cudaFuncAttributes fa{};
+      BB_CUDA_TRY(cudaFuncGetAttributes(&fa, kernel));
+      if (fa.numRegs * C::THREADS < 128 * C::CTRL_REGS + 256 * C::EPI_REGS) {
+        set_error("bb_linear: kernel built with %d registers per thread; its register split needs %d", fa.numRegs,
+                  kLaunchRegs);
+        return BB_ERR_INTERNAL;
+      }
+    }
+    int rc = allow_smem(kernel, C::SMEM_BYTES, pl.device, done);
+    if (rc != BB_OK) return rc;
+  }
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = config(pl.grid, C::THREADS, C::SMEM_BYTES, kCG, pl.stream, attr);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, pl.tm_a, pl.tm_b, pl.tm_sfa, pl.tm_sfb, pl.tm_d, pl.tile),
+                    "launch bb_lowp_gemm_kernel");
+}
+
+// CTA pairs resident at once (SMs that have no partner in their GPC stay idle).
+template <int kKind>
+int resident_pairs(const bb_linear_plan& pl, int sm_count, int* pairs) {
+  using C = Cfg<kKind, 2>;
+  static int known[kMaxDevices] = {};
+  if (pl.device < kMaxDevices && known[pl.device]) {
+    *pairs = known[pl.device];
+    return BB_OK;
+  }
+  static bool done[kMaxDevices] = {};
+  auto kernel = bb_lowp_gemm_kernel<kKind, 2, true, false>;
+  int rc = allow_smem(kernel, C::SMEM_BYTES, pl.device, done);
+  if (rc != BB_OK) return rc;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = config(sm_count / 2 * 2, C::THREADS, C::SMEM_BYTES, 2, pl.stream, attr);
+  int n = 0;
+  BB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+  *pairs = n > 0 && n < sm_count / 2 ? n : sm_count / 2;
+  if (pl.device < kMaxDevices) known[pl.device] = *pairs;
+  return BB_OK;
+}
+
+template <int kKind>
+int launch_kind(const bb_linear_plan& pl) {
+  if (pl.few) return launch_few_kind<kKind>(pl);
+  if (pl.cg == 2) return pl.direct ? launch_tile<kKind, 2, true>(pl) : launch_tile<kKind, 2, false>(pl);
+  return pl.direct ? launch_tile<kKind, 1, true>(pl) : launch_tile<kKind, 1, false>(pl);
+}
+
+int launch_linear(const bb_linear_plan& pl) {
+  if (pl.kind == kNvfp4) return launch_kind<kNvfp4>(pl);
+  if (pl.kind == kMxfp4) return launch_kind<kMxfp4>(pl);
+  return launch_kind<kFp8Group>(pl);
+}
+
+// K splits of the few-rows kernel: enough CTAs to fill the SMs at the tile's
+// residency, each with at least two stages of K, up to a portable cluster.
+int choose_splits(int units, int k_stages, int slots) {
+  int s = slots / (units > 0 ? units : 1);
+  if (s > 8) s = 8;
+  if (s > k_stages / 2) s = k_stages / 2;
+  return s < 1 ? 1 : s;
+}
+
+template <int kKind>
+void few_info(int tn, bb_lowp_info* info) {
+  auto set = [&](auto cfg) {
+    using C = decltype(cfg);
+    info->stages = C::STAGES;
+    info->smem_bytes = C::SMEM_BYTES;
+    info->tmem_columns = C::TMEM;
+    info->threads_per_cta = C::THREADS;
+  };
+  switch (tn) {
+    case 16: set(FewCfg<kKind, 16>{}); break;
+    case 32: set(FewCfg<kKind, 32>{}); break;
+    case 64: set(FewCfg<kKind, 64>{}); break;
+    case 128: set(FewCfg<kKind, 128>{}); break;
+    default: set(FewCfg<kKind, 256>{}); break;
+  }
+}
+
+template <int kKind>
+void tile_info(int cg, bb_lowp_info* info) {
+  info->stages = cg == 2 ? Cfg<kKind, 2>::STAGES : Cfg<kKind, 1>::STAGES;
+  info->smem_bytes = cg == 2 ? Cfg<kKind, 2>::SMEM_BYTES : Cfg<kKind, 1>::SMEM_BYTES;
+  info->tmem_columns = TMEM_COLS;
+  info->threads_per_cta = Cfg<kKind, 1>::THREADS;
+}
+
+// The operands' tensor maps: 128-byte K rows of `box_rows` rows, and the scale
+// atoms as rows of 8-byte words (one row per 128 operand rows).
+int map_rows(CUtensorMap* tm, const void* data, int64_t row_bytes, int64_t rows, int box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(row_bytes), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(row_bytes)};
+  const uint32_t box[2] = {ROW_BYTES, static_cast<uint32_t>(box_rows)};
+  return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 2, data, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+int map_atoms(CUtensorMap* tm, const void* atoms, int64_t atoms_k, int64_t blocks, int stage_atoms, int box_blocks) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(atoms_k) * 64, static_cast<uint64_t>(blocks)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(atoms_k) * 512};
+  const uint32_t box[2] = {static_cast<uint32_t>(stage_atoms) * 64, static_cast<uint32_t>(box_blocks)};
+  return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_UINT64, 8, 2, atoms, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -159,12 +608,13 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
       return BB_ERR_ARGUMENT;
     }
     auto off = [](const void* ptr, size_t to) { return reinterpret_cast<uintptr_t>(ptr) % to != 0; };
-    if (off(a, 16) || off(b, 16) || off(sfa, fp8 ? 4 : 16) || off(sfb, fp8 ? 4 : 16) ||
-        off(d, d_dtype == BB_DTYPE_F32 ? 4 : 2) || off(scale_a_dev, 4) || off(scale_b_dev, 4)) {
+    const size_t d_size = d_dtype == BB_DTYPE_F32 ? 4 : 2;
+    if (off(a, 16) || off(b, 16) || off(sfa, fp8 ? 4 : 16) || off(sfb, fp8 ? 4 : 16) || off(d, d_size) ||
+        off(scale_a_dev, 4) || off(scale_b_dev, 4)) {
       set_error("bb_linear_plan_create: operands must be 16-byte aligned (FP8 scales 4), D to its type");
       return BB_ERR_ARGUMENT;
     }
-    if (((m + 63) / 64) * ((n + 63) / 64) > 0x7fffffff) {
+    if (((m + 127) / 128) * ((n + 127) / 128) > 0x0fffffff) {
       set_error("bb_linear_plan_create: M=%lld x N=%lld is more than one launch covers", (long long)m, (long long)n);
       return BB_ERR_ARGUMENT;
     }
@@ -179,32 +629,120 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
     h->kind = kind;
     h->device = dev.device;
     h->stream = static_cast<cudaStream_t>(stream);
-    SimpleParams& p = h->params;
-    p.m = static_cast<int32_t>(m);
-    p.n = static_cast<int32_t>(n);
-    p.k = static_cast<int32_t>(k);
-    p.atoms_k = static_cast<int32_t>(kind == BB_LOWP_NVFP4 ? (k + 63) / 64 : (k + 127) / 128);
-    p.a = static_cast<const uint8_t*>(a);
-    p.b = static_cast<const uint8_t*>(b);
-    p.sfa = static_cast<const uint8_t*>(sfa);
-    p.sfb = static_cast<const uint8_t*>(sfb);
-    p.sfa_ld = sfa_ld;
-    p.ldd = ldd;
-    p.scale_a = scale_a;
-    p.scale_b = scale_b;
-    p.scale_a_dev = scale_a_dev;
-    p.scale_b_dev = scale_b_dev;
-    p.d = d;
-    p.d_dtype = d_dtype;
+    const int64_t row_bytes = fp8 ? k : k / 2;
+    const int64_t atoms_k = kind == BB_LOWP_NVFP4 ? (k + 63) / 64 : (k + 127) / 128;
+    const int stage_atoms = kind == BB_LOWP_NVFP4 ? 4 : 2;
+    const int64_t rb_m = (m + 127) / 128, rb_n = (n + 127) / 128;
+    const int k_stages = static_cast<int>((row_bytes + ROW_BYTES - 1) / ROW_BYTES);
+    h->few = m <= 256;
+    if (h->few) {
+      h->tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
+      FewParams& p = h->fp;
+      p.m = static_cast<int32_t>(m);
+      p.n = static_cast<int32_t>(n);
+      p.k_stages = k_stages;
+      p.tiles_n = static_cast<int32_t>(rb_n);
+      const int units = static_cast<int>(rb_n * ((m + h->tn - 1) / h->tn));
+      p.splits = choose_splits(units, k_stages, dev.sm_count * (h->tn <= 128 ? 2 : 1));
+      p.kb = static_cast<int32_t>((k + 127) / 128);
+      p.sfa = static_cast<const float*>(sfa);
+      p.sfb = static_cast<const float*>(sfb);
+      p.sfa_ld = sfa_ld;
+      p.ldd = ldd;
+      p.scale = (scale_a_dev ? 1.f : scale_a) * (scale_b_dev ? 1.f : scale_b);
+      p.scale_dev[0] = scale_a_dev;
+      p.scale_dev[1] = scale_b_dev;
+      p.d = d;
+      p.d_dtype = d_dtype;
+      h->grid = units * p.splits;
+    } else {
+      h->cg = 2;
+      Params& p = h->tile;
+      const int tile_m = BM * h->cg;
+      p.m = static_cast<int32_t>(m);
+      p.n = static_cast<int32_t>(n);
+      p.k = static_cast<int32_t>(k);
+      p.tiles_m = static_cast<int32_t>((m + tile_m - 1) / tile_m);
+      p.tiles_n = static_cast<int32_t>((n + 255) / 256);
+      p.num_tiles = p.tiles_m * p.tiles_n;
+      p.k_stages = k_stages;
+      p.rb_m = static_cast<int32_t>(rb_m);
+      p.rb_n = static_cast<int32_t>(rb_n);
+      const int64_t g = kGroupABytes / (tile_m * row_bytes);
+      p.group_m = static_cast<int32_t>(g < 1 ? 1 : g > p.tiles_m ? p.tiles_m : g);
+      int clusters = 0;
+      rc = kind == kNvfp4   ? resident_pairs<kNvfp4>(*h, dev.sm_count, &clusters)
+           : kind == kMxfp4 ? resident_pairs<kMxfp4>(*h, dev.sm_count, &clusters)
+                            : resident_pairs<kFp8Group>(*h, dev.sm_count, &clusters);
+      if (rc != BB_OK) {
+        delete h;
+        return rc;
+      }
+      p.num_clusters = p.num_tiles < clusters ? p.num_tiles : clusters;
+      p.sfa = static_cast<const uint8_t*>(sfa);
+      p.sfb = static_cast<const uint8_t*>(sfb);
+      p.global_scale = (scale_a_dev ? 1.f : scale_a) * (scale_b_dev ? 1.f : scale_b);
+      p.scale_dev[0] = scale_a_dev;
+      p.scale_dev[1] = scale_b_dev;
+      p.sfa_ld = sfa_ld;
+      p.ldd = ldd;
+      p.d = static_cast<__nv_bfloat16*>(d);
+      p.d_dtype = d_dtype;
+      const bool rows16 = reinterpret_cast<uintptr_t>(d) % 16 == 0 && (ldd * d_size) % 16 == 0;
+      p.d_vec = rows16;
+      // TMA stores want 16-byte rows; other types and strides are written from registers.
+      h->direct = d_dtype != BB_DTYPE_BF16 || !rows16;
+      h->grid = p.num_clusters * h->cg;
+    }
+    if (m > 0) {
+      const int box_a = h->few ? h->tn : BM, box_b = h->few ? 128 : 256 / h->cg;
+      rc = map_rows(&h->tm_a, a, row_bytes, m, box_a);
+      if (rc == BB_OK) rc = map_rows(&h->tm_b, b, row_bytes, n, box_b);
+      if (fp8) {
+        h->tm_sfa = h->tm_a;  // unused: FP32 scales do not travel by TMA
+        h->tm_sfb = h->tm_b;
+      } else {
+        if (rc == BB_OK) rc = map_atoms(&h->tm_sfa, sfa, atoms_k, rb_m, stage_atoms, h->few && h->tn > 128 ? 2 : 1);
+        if (rc == BB_OK) rc = map_atoms(&h->tm_sfb, sfb, atoms_k, rb_n, stage_atoms, h->few ? 1 : 2);
+      }
+      h->tm_d = h->tm_a;
+      if (rc == BB_OK && !h->few && !h->direct) {
+        const uint64_t dims[2] = {static_cast<uint64_t>(n), static_cast<uint64_t>(m)};
+        const uint64_t strides[1] = {static_cast<uint64_t>(ldd) * 2};
+        const uint32_t box[2] = {64, 32};
+        rc = encode_tiled(&h->tm_d, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 2, d, dims, strides, box,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
+      }
+      if (rc == BB_OK) rc = check_cuda(cudaMalloc(&h->status_dev, sizeof(int)), "cudaMalloc(status)");
+      if (rc == BB_OK) rc = check_cuda(cudaMemset(h->status_dev, 0, sizeof(int)), "cudaMemset(status)");
+      if (rc != BB_OK) {
+        if (h->status_dev) cudaFree(h->status_dev);
+        delete h;
+        return rc;
+      }
+    }
+    h->fp.status = h->tile.status = h->status_dev;
     if (info) {
       *info = bb_lowp_info{};
       info->kind = kind;
-      info->tile_m = 64;
-      info->tile_n = 64;
-      info->tile_k = 32;
-      info->threads_per_cta = 256;
-      info->num_tiles = ((m + 63) / 64) * ((n + 63) / 64);
-      info->grid_ctas = info->num_tiles;
+      info->tile_m = h->few ? h->tn : BM * h->cg;
+      info->tile_n = h->few ? 128 : 256;
+      info->tile_k = fp8 ? 128 : 256;
+      info->grid_ctas = m > 0 ? h->grid : 0;
+      info->cta_group = h->cg;
+      if (h->few) {
+        info->num_tiles = h->grid / h->fp.splits;
+        if (kind == kNvfp4) few_info<kNvfp4>(h->tn, info);
+        else if (kind == kMxfp4) few_info<kMxfp4>(h->tn, info);
+        else few_info<kFp8Group>(h->tn, info);
+      } else {
+        info->num_tiles = h->tile.num_tiles;
+        if (kind == kNvfp4) tile_info<kNvfp4>(h->cg, info);
+        else if (kind == kMxfp4) tile_info<kMxfp4>(h->cg, info);
+        else tile_info<kFp8Group>(h->cg, info);
+      }
+      info->reserved[0] = h->few ? 1 : 0;
+      info->reserved[1] = h->few ? h->fp.splits : 1;
     }
     *plan = h;
     return BB_OK;
@@ -220,16 +758,11 @@ BB_API int bb_linear_execute_n(bb_linear_plan* plan, int iterations) {
       set_error("bb_linear_execute_n: null plan or negative iteration count");
       return BB_ERR_ARGUMENT;
     }
-    const SimpleParams& p = plan->params;
-    if (p.m == 0) return BB_OK;
+    if (!plan->status_dev) return BB_OK;  // no rows
     DeviceGuard guard(plan->device);
     BB_CUDA_TRY(guard.status);
     for (int i = 0; i < iterations; ++i) {
-      const unsigned grid = static_cast<unsigned>((p.n + 63) / 64) * ((p.m + 63) / 64);
-      if (plan->kind == BB_LOWP_NVFP4) simple_linear_kernel<BB_LOWP_NVFP4><<<grid, 256, 0, plan->stream>>>(p);
-      else if (plan->kind == BB_LOWP_MXFP4) simple_linear_kernel<BB_LOWP_MXFP4><<<grid, 256, 0, plan->stream>>>(p);
-      else simple_linear_kernel<BB_LOWP_FP8_GROUP128><<<grid, 256, 0, plan->stream>>>(p);
-      int rc = check_cuda(cudaGetLastError(), "launch simple_linear_kernel");
+      int rc = launch_linear(*plan);
       if (rc != BB_OK) return rc;
       ++plan->launches;
       g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
@@ -242,18 +775,35 @@ BB_API int bb_linear_execute_n(bb_linear_plan* plan, int iterations) {
 }
 
 BB_API int bb_linear_synchronize(bb_linear_plan* plan) {
-  if (!plan) {
-    set_error("bb_linear_synchronize: null plan");
-    return BB_ERR_ARGUMENT;
+  try {
+    if (!plan) {
+      set_error("bb_linear_synchronize: null plan");
+      return BB_ERR_ARGUMENT;
+    }
+    BB_CUDA_TRY(cudaStreamSynchronize(plan->stream));
+    if (!plan->status_dev) return BB_OK;
+    int st = 0;
+    BB_CUDA_TRY(cudaMemcpy(&st, plan->status_dev, sizeof(int), cudaMemcpyDeviceToHost));
+    if (st != 0) {
+      set_error("linear kernel reported device status 0x%x (%s)", st,
+                st == kDevBadLaunch ? "launch contract violated" : "a bounded wait timed out");
+      return st == kDevBadLaunch ? BB_ERR_INTERNAL : BB_ERR_TIMEOUT;
+    }
+    return BB_OK;
+  } catch (...) {
+    set_error("bb_linear_synchronize: unexpected C++ exception");
+    return BB_ERR_INTERNAL;
   }
-  return check_cuda(cudaStreamSynchronize(plan->stream), "cudaStreamSynchronize");
 }
 
 BB_API int64_t bb_linear_launches(const bb_linear_plan* plan) { return plan ? plan->launches : -1; }
 
 BB_API int bb_linear_destroy(bb_linear_plan* plan) {
+  if (!plan) return BB_OK;
+  int rc = BB_OK;
+  if (plan->status_dev) rc = check_cuda(cudaFree(plan->status_dev), "cudaFree(status)");
   delete plan;
-  return BB_OK;
+  return rc;
 }
 
 }  // extern "C"
