@@ -442,6 +442,10 @@ __global__ void __launch_bounds__(Cfg<kKind, kCG>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const int cluster_idx = blockIdx.x / kCG;
+  if constexpr (kLinear) {
+    grid_wait();
+    grid_trigger();
+  }
 
   if (warp < C::EPI_W0) {
     if constexpr (C::kRegSplit) {

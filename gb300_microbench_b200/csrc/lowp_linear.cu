@@ -63,9 +63,11 @@ struct FewCfg {
   static_assert(BUFS < STAGES, "a stage's barrier tells the epilogue of its block");
 };
 
+constexpr int kMaxSplits = 8;  // the portable cluster size
+
 struct FewParams {
   int32_t m, n;
-  int32_t k_stages, splits, tiles_n;
+  int32_t k_stages, splits;
   int32_t kb;          // FP8: K blocks
   const float* sfa;    // FP8: [kb][sfa_ld]
   const float* sfb;    // FP8: [n blocks][kb]
@@ -100,9 +102,12 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t* r) {
   }
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_v4f(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
   return v;
 }
 
@@ -129,8 +134,7 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int unit = blockIdx.x / p.splits;  // (token tile, weight row block)
-  const int m0 = unit / p.tiles_n * C::TN, n_blk = unit % p.tiles_n;
+  const int n_blk = blockIdx.x / p.splits;
   const int ks0 = static_cast<int>(static_cast<int64_t>(p.k_stages) * rank / p.splits);
   const int ks1 = static_cast<int>(static_cast<int64_t>(p.k_stages) * (rank + 1) / p.splits);
 
@@ -158,6 +162,16 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
+  // All of the above overlaps the end of the kernel before. The weights may
+  // come from that kernel too, so before the wait they are fetched into L2
+  // only, where its writes land as well.
+  if (warp == 0 && elect_one()) {
+    for (int ks = ks0; ks < ks1 && ks < ks0 + STAGES; ++ks) tma_prefetch_2d(&tm_w, ks * ROW_BYTES, n_blk * 128);
+  }
+  __syncwarp();
+  grid_wait();
+  grid_trigger();
+
   float scale = p.scale;
   float* red = reinterpret_cast<float*>(smem);  // [TN][128] partial sums, over the ring once it is idle
   const int q = warp & 3, half = (warp - 2) / 4;
@@ -165,8 +179,7 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
   const int col0 = half * C::COLS;     // first token of this thread (epilogue)
   const int n = n_blk * 128 + row;
   auto put = [&](int c, float v) {
-    const int m = m0 + c;
-    if (m < p.m && n < p.n) store_one(p.d, p.d_dtype, m * p.ldd + n, v * scale);
+    if (c < p.m && n < p.n) store_one(p.d, p.d_dtype, c * p.ldd + n, v * scale);
   };
 
   if (warp == 0) {
@@ -182,10 +195,10 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
         const uint32_t fb = smem_u32(&full[stage]);
         mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
         tma_load_2d(smem_u32(smem_w + stage * C::W_BYTES), &tm_w, fb, ks * ROW_BYTES, n_blk * 128);
-        tma_load_2d(smem_u32(smem_x + stage * C::X_BYTES), &tm_x, fb, ks * ROW_BYTES, m0);
+        tma_load_2d(smem_u32(smem_x + stage * C::X_BYTES), &tm_x, fb, ks * ROW_BYTES, 0);
         if constexpr (C::FP4) {
           tma_load_2d(smem_u32(smem_sfw + stage * C::SFW_BYTES), &tm_sfw, fb, ks * 64 * C::ATOMS, n_blk);
-          tma_load_2d(smem_u32(smem_sfx + stage * C::SFX_BYTES), &tm_sfx, fb, ks * 64 * C::ATOMS, m0 / 128);
+          tma_load_2d(smem_u32(smem_sfx + stage * C::SFX_BYTES), &tm_sfx, fb, ks * 64 * C::ATOMS, 0);
         }
       }
       __syncwarp();
@@ -241,12 +254,10 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
                 tmem_cp_desc<1>(t_x + 4 * b, sfx + (b * C::ATOMS + a) * (SF_ATOM >> 4));
             }
             const uint32_t acc = (it | g) != 0 ? 1u : 0u;
-            // A 64-token tile may begin in the middle of a 128-row scale block: 32 rows a column.
-            const uint32_t t_xs = t_x + static_cast<uint32_t>(m0 % 128) / 32;
             if constexpr (kKind == kNvfp4)
-              mma_nvf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_nvf4(128, C::TN), t_w, t_xs, acc);
+              mma_nvf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_nvf4(128, C::TN), t_w, t_x, acc);
             else
-              mma_mxf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_mxf4(128, C::TN, 2 * (g % 2)), t_w, t_xs, acc);
+              mma_mxf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_mxf4(128, C::TN, 2 * (g % 2)), t_w, t_x, acc);
           }
         } else {
 #pragma unroll
@@ -283,24 +294,35 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
       for (int c = 0; c < C::COLS; ++c) acc[c] = 0.f;
       float* my_scale = smem_scale + (warp - 2) * C::COLS;  // this warp's token scales of the current K block
       constexpr int kPer = (C::COLS + 31) / 32;
-      float next[kPer], next_b = 0.f;
-      auto load = [&](int kb) {
+      // The lane's token scales times the weights' scale of the next kAhead K
+      // blocks: a load takes up to 800 ns, a block of weights half of that.
+      constexpr int kAhead = 4;
+      float next[kAhead][kPer], next_b[kAhead];
+      auto load = [&](int slot, int kb) {
+        if (kb >= ks1) return;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
           const int c = lane + 32 * j;
-          next[j] = c < C::COLS && m0 + col0 + c < p.m ? __ldg(p.sfa + kb * p.sfa_ld + m0 + col0 + c) : 0.f;
+          next[slot][j] = c < C::COLS && col0 + c < p.m ? __ldg(p.sfa + kb * p.sfa_ld + col0 + c) : 0.f;
         }
-        next_b = __ldg(p.sfb + static_cast<int64_t>(n_blk) * p.kb + kb);
+        next_b[slot] = __ldg(p.sfb + static_cast<int64_t>(n_blk) * p.kb + kb);
       };
-      load(ks0);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) load(j, ks0 + j);
       for (int ks = ks0; ks < ks1; ++ks) {
         const uint32_t it = ks - ks0, buf = it % C::BUFS;
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
-          if (lane + 32 * j < C::COLS) my_scale[lane + 32 * j] = next[j] * next_b;
+          if (lane + 32 * j < C::COLS) my_scale[lane + 32 * j] = next[0][j] * next_b[0];
         __syncwarp();
-        if (ks + 1 < ks1) load(ks + 1);
+#pragma unroll
+        for (int i = 0; i + 1 < kAhead; ++i) {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) next[i][j] = next[i + 1][j];
+          next_b[i] = next_b[i + 1];
+        }
+        load(kAhead - 1, ks + kAhead);
         // The commit that releases the operand stage also says that the K
         // block's partial is complete; the MMA warp runs at most BUFS < STAGES
         // blocks ahead, so the parity cannot be overtaken.
@@ -341,7 +363,7 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
         // The ring is idle (`done`): no copy is in flight and every MMA has read its operands.
 #pragma unroll
         for (int c = 0; c < C::COLS; ++c)
-          if (m0 + col0 + c < p.m) red[(col0 + c) * 128 + row] = acc[c];
+          if (col0 + c < p.m) red[(col0 + c) * 128 + row] = acc[c];
       }
     }
   }
@@ -349,13 +371,41 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
     __syncwarp();
     cluster_sync();
     if (warp >= 2) {
-      // Rank r adds the tokens r, r + splits, ... of all ranks' partial sums.
-      const int tokens = min(C::TN, p.m - m0);
-      const uint32_t base = smem_u32(red) + row * 4;
-      for (int c = rank + half * p.splits; c < tokens; c += p.splits * (C::EPI_W / 4)) {
-        float v = 0.f;
-        for (int r = 0; r < p.splits; ++r) v += ld_cluster_f32(mapa_shared(base + c * 512, r));
-        put(c, v);
+      // Rank r adds the tokens r, r + splits, ... of all ranks' partial sums: a
+      // warp per token, a lane four weight rows. Remote loads take most of a
+      // microsecond each, so those of all ranks and of kBatch tokens are in flight together.
+      constexpr int kBatch = C::TN <= 16 ? 1 : 2;
+      const uint32_t base = smem_u32(red) + lane * 16;
+      const int n4 = n_blk * 128 + lane * 4;
+      for (int c = rank + (warp - 2) * p.splits; c < p.m; c += p.splits * C::EPI_W * kBatch) {
+        float4 v[kBatch][kMaxSplits];
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) {
+          if (r >= p.splits) break;
+          const uint32_t from = mapa_shared(base + c * 512, r);
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j)
+            if (c + j * p.splits * C::EPI_W < p.m) v[j][r] = ld_cluster_v4f(from + j * p.splits * C::EPI_W * 512);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int token = c + j * p.splits * C::EPI_W;
+          if (token >= p.m) break;
+          float4 sum = v[j][0];
+#pragma unroll
+          for (int r = 1; r < kMaxSplits; ++r) {
+            if (r >= p.splits) break;
+            sum.x += v[j][r].x;
+            sum.y += v[j][r].y;
+            sum.z += v[j][r].z;
+            sum.w += v[j][r].w;
+          }
+          const int64_t at = token * p.ldd + n4;
+          const float out[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n4 + i < p.n) store_one(p.d, p.d_dtype, at + i, out[i]);
+        }
       }
     }
     __syncwarp();
@@ -404,7 +454,8 @@ int allow_smem(K kernel, int bytes, int device, bool (&done)[kMaxDevices]) {
   return BB_OK;
 }
 
-cudaLaunchConfig_t config(int grid, int threads, int smem, int cluster, cudaStream_t stream, cudaLaunchAttribute* attr) {
+cudaLaunchConfig_t config(int grid, int threads, int smem, int cluster, bool dependent, cudaStream_t stream,
+                          cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
@@ -414,8 +465,10 @@ cudaLaunchConfig_t config(int grid, int threads, int smem, int cluster, cudaStre
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = dependent ? 2 : 1;
   return cfg;
 }
 
@@ -426,8 +479,8 @@ int launch_few(const bb_linear_plan& pl) {
   auto kernel = few_rows_kernel<kKind, kTN>;
   int rc = allow_smem(kernel, C::SMEM_BYTES, pl.device, done);
   if (rc != BB_OK) return rc;
-  cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg = config(pl.grid, C::THREADS, C::SMEM_BYTES, pl.fp.splits, pl.stream, attr);
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = config(pl.grid, C::THREADS, C::SMEM_BYTES, pl.fp.splits, true, pl.stream, attr);
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, pl.tm_b, pl.tm_a, pl.tm_sfb, pl.tm_sfa, pl.fp),
                     "launch few_rows_kernel");
 }
@@ -463,8 +516,8 @@ int launch_tile(const bb_linear_plan& pl) {
     int rc = allow_smem(kernel, C::SMEM_BYTES, pl.device, done);
     if (rc != BB_OK) return rc;
   }
-  cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg = config(pl.grid, C::THREADS, C::SMEM_BYTES, kCG, pl.stream, attr);
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = config(pl.grid, C::THREADS, C::SMEM_BYTES, kCG, true, pl.stream, attr);
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, pl.tm_a, pl.tm_b, pl.tm_sfa, pl.tm_sfb, pl.tm_d, pl.tile),
                     "launch bb_lowp_gemm_kernel");
 }
@@ -482,8 +535,8 @@ int resident_pairs(const bb_linear_plan& pl, int sm_count, int* pairs) {
   auto kernel = bb_lowp_gemm_kernel<kKind, 2, true, false>;
   int rc = allow_smem(kernel, C::SMEM_BYTES, pl.device, done);
   if (rc != BB_OK) return rc;
-  cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t cfg = config(sm_count / 2 * 2, C::THREADS, C::SMEM_BYTES, 2, pl.stream, attr);
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = config(sm_count / 2 * 2, C::THREADS, C::SMEM_BYTES, 2, false, pl.stream, attr);
   int n = 0;
   BB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
   *pairs = n > 0 && n < sm_count / 2 ? n : sm_count / 2;
@@ -504,12 +557,19 @@ int launch_linear(const bb_linear_plan& pl) {
   return launch_kind<kFp8Group>(pl);
 }
 
-// K splits of the few-rows kernel: enough CTAs to fill the SMs at the tile's
-// residency, each with at least two stages of K, up to a portable cluster.
-int choose_splits(int units, int k_stages, int slots) {
-  int s = slots / (units > 0 ? units : 1);
-  if (s > 8) s = 8;
-  if (s > k_stages / 2) s = k_stages / 2;
+// K splits of the few-rows kernel. One CTA per SM suffices for a short K: more
+// of them only add to the exchange (MXFP4 128 x 4096 x 4096, 32 row blocks:
+// 4 splits 8.4 us, 8 splits 13.3). A second CTA per SM keeps more of a long
+// weight stream in flight (NVFP4 1 x 8192 x 8192: 2 splits 10.7 us, 4 splits
+// 9.2; FP8 1 x 14336 x 4096: 1 split 14.4, 2 splits 13.3) where each still has
+// kLongShare stages. Never more CTAs than are resident at once: a second wave
+// costs half the kernel (5 splits of the same NVFP4 case 14.2 us).
+constexpr int kLongShare = 8;
+int choose_splits(int units, int k_stages, int sm_count, int ctas_per_sm) {
+  auto within = [](int s, int most) { return s < most ? s : most; };
+  int s = within(within(sm_count / units, kMaxSplits), k_stages / 2);
+  const int more = within(within(sm_count * ctas_per_sm / units, kMaxSplits), k_stages / kLongShare);
+  if (more > s) s = more;
   return s < 1 ? 1 : s;
 }
 
@@ -641,9 +701,8 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
       p.m = static_cast<int32_t>(m);
       p.n = static_cast<int32_t>(n);
       p.k_stages = k_stages;
-      p.tiles_n = static_cast<int32_t>(rb_n);
-      const int units = static_cast<int>(rb_n * ((m + h->tn - 1) / h->tn));
-      p.splits = choose_splits(units, k_stages, dev.sm_count * (h->tn <= 128 ? 2 : 1));
+      const int units = static_cast<int>(rb_n);
+      p.splits = choose_splits(units, k_stages, dev.sm_count, h->tn <= 128 ? 2 : 1);
       p.kb = static_cast<int32_t>((k + 127) / 128);
       p.sfa = static_cast<const float*>(sfa);
       p.sfb = static_cast<const float*>(sfb);

@@ -104,6 +104,16 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
   return r;
 }
 
+// ---------------------------------------------------------------- dependent launches
+// A kernel launched with programmatic stream serialization starts while the
+// one before it still runs: grid_wait() waits until that one has completed and
+// its writes are visible (at once when there is none), and stands before the
+// first access to memory another kernel may write or read. grid_trigger()
+// lets the next such kernel start; every CTA of a kernel launched so waits
+// before it ends, so completion stays transitive along the stream.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint32_t addr, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(addr), "r"(count) : "memory");
@@ -302,6 +312,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint
       " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
       "l"(tmap), "r"(mbar), "r"(x), "r"(y)
       : "memory");
+}
+// The same box into L2 only.
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tmap), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t mbar, int32_t x,
                                             int32_t y, int32_t z) {

@@ -22,6 +22,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace bb {
 extern std::atomic<int64_t> g_kernel_launches;
@@ -138,6 +139,8 @@ constexpr int kNormMaxIters = 8;  // 8 vectors of 8 columns per thread: 65536 co
 template <typename T, int kIters, bool kWide>
 __global__ void __launch_bounds__(kNormMaxThreads) rmsnorm_fp8_kernel(const NormParams p) {
   __shared__ float warp_sum[32];
+  grid_wait();
+  grid_trigger();
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.res_ld : nullptr;
@@ -283,6 +286,8 @@ __device__ __forceinline__ float found_scale(const float* partial, int n) {
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(kFp4Threads) absmax_kernel(const Fp4Params p, float* partial) {
   __shared__ uint32_t warp_max[kFp4Threads / 32];
+  grid_wait();
+  grid_trigger();
   const int vecs = (p.cols + 7) / 8;
   uint32_t m = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -307,6 +312,8 @@ __global__ void __launch_bounds__(kFp4Threads) absmax_kernel(const Fp4Params p, 
 // make the 4 bytes a row has in one atom.
 template <typename T, bool kMx, bool kWide>
 __global__ void __launch_bounds__(kFp4Threads) fp4_quant_kernel(const Fp4Params p) {
+  grid_wait();
+  grid_trigger();
   float g = p.tensor_scale;
   if constexpr (!kMx) {
     if (p.partial_max) {
@@ -423,31 +430,43 @@ bool aligned16(const void* p, int64_t ld, size_t size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (static_cast<size_t>(ld) * size) % 16 == 0;
 }
 
+// Every launch may start before the one before it has ended (the kernels wait).
+template <typename... Args, typename... Given>
+cudaError_t launch(void (*kernel)(Args...), unsigned grid, int threads, cudaStream_t stream, Given... given) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, given...);
+}
+
 template <typename T, bool kWide>
 cudaError_t launch_norm(const bb_quant_plan& pl) {
-  const dim3 grid(static_cast<unsigned>(pl.np.rows)), block(pl.threads);
+  const unsigned grid = static_cast<unsigned>(pl.np.rows);
   switch (pl.iters) {
-    case 1: rmsnorm_fp8_kernel<T, 1, kWide><<<grid, block, 0, pl.stream>>>(pl.np); break;
-    case 2: rmsnorm_fp8_kernel<T, 2, kWide><<<grid, block, 0, pl.stream>>>(pl.np); break;
-    case 4: rmsnorm_fp8_kernel<T, 4, kWide><<<grid, block, 0, pl.stream>>>(pl.np); break;
-    default: rmsnorm_fp8_kernel<T, 8, kWide><<<grid, block, 0, pl.stream>>>(pl.np); break;
+    case 1: return launch(rmsnorm_fp8_kernel<T, 1, kWide>, grid, pl.threads, pl.stream, pl.np);
+    case 2: return launch(rmsnorm_fp8_kernel<T, 2, kWide>, grid, pl.threads, pl.stream, pl.np);
+    case 4: return launch(rmsnorm_fp8_kernel<T, 4, kWide>, grid, pl.threads, pl.stream, pl.np);
+    default: return launch(rmsnorm_fp8_kernel<T, 8, kWide>, grid, pl.threads, pl.stream, pl.np);
   }
-  return cudaGetLastError();
 }
 
 template <typename T, bool kWide>
 cudaError_t launch_fp4(const bb_quant_plan& pl) {
   const bool mx = pl.fmt == BB_LOWP_MXFP4;
   if (pl.partials) {
-    absmax_kernel<T, kWide><<<pl.partials, kFp4Threads, 0, pl.stream>>>(pl.fp, pl.partial);
-    cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch(absmax_kernel<T, kWide>, pl.partials, kFp4Threads, pl.stream, pl.fp, pl.partial);
     if (e != cudaSuccess) return e;
   }
   const int64_t total = pl.fp.rows_pad * pl.fp.atoms_k * (mx ? 8 : 4);
   const unsigned grid = static_cast<unsigned>((total + kFp4Threads - 1) / kFp4Threads);
-  if (mx) fp4_quant_kernel<T, true, kWide><<<grid, kFp4Threads, 0, pl.stream>>>(pl.fp);
-  else fp4_quant_kernel<T, false, kWide><<<grid, kFp4Threads, 0, pl.stream>>>(pl.fp);
-  return cudaGetLastError();
+  return mx ? launch(fp4_quant_kernel<T, true, kWide>, grid, kFp4Threads, pl.stream, pl.fp)
+            : launch(fp4_quant_kernel<T, false, kWide>, grid, kFp4Threads, pl.stream, pl.fp);
 }
 
 template <typename T>
