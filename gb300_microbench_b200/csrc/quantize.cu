@@ -20,6 +20,7 @@
 
 #include <atomic>
 #include <new>
+#include <type_traits>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -91,28 +92,48 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// y / s for many y of one s, correctly rounded: with r = 1 / s correctly
-// rounded, one residual step q = q0 + (y - q0 s) r of q0 = y r gives the
-// rounded quotient (Markstein, IBM J. Res. Dev. 34, 1990) while nothing leaves
-// the normal numbers; `plain` (s or 1 / s outside 2^+-60) divides instead.
-// Three FP32 instructions per element instead of a division's dozen: the
-// quantisers would be bound by it otherwise.
-struct Divider {
-  float s, r;
-  bool plain;
-  __device__ __forceinline__ float operator()(float y) const {
-    if (plain) return __fdiv_rn(y, s);
-    const float q0 = y * r;
-    const float q = __fmaf_rn(__fmaf_rn(-q0, s, y), r, q0);
-    return fabsf(q0) < 0x1p60f ? q : q0;  // an infinite y has no residual
-  }
+// Two FP32 operations per instruction (sm_100's packed FP32).
+struct F2 {
+  uint64_t v;
 };
-__device__ __forceinline__ Divider divider(float s) {
-  Divider d;
-  d.s = s;
-  d.r = __fdiv_rn(1.f, s);
-  d.plain = !(s > 0x1p-60f && s < 0x1p60f);
-  return d;
+__device__ __forceinline__ F2 pack2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// y[i] / s for the N values of a block whose magnitudes are at most `most`,
+// correctly rounded: with r = 1 / s correctly rounded, one residual step
+// q = q0 + (y - q0 s) r of q0 = y r gives the rounded quotient (Markstein, IBM
+// J. Res. Dev. 34, 1990) while nothing leaves the normal numbers; other blocks
+// divide. One and a half instructions per value instead of a division's dozen,
+// which would bound the quantisers.
+template <int N>
+__device__ __forceinline__ void divide(float (&y)[N], float s, float most) {
+  const float r = __fdiv_rn(1.f, s);
+  if (s > 0x1p-60f && s < 0x1p60f && most * r < 0x1p60f) {
+    const F2 r2 = pack2(r, r), s2 = pack2(-s, -s);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const F2 v = pack2(y[i], y[i + 1]);
+      const F2 q0 = mul2(v, r2);
+      unpack2(fma2(fma2(q0, s2, v), r2, q0), y[i], y[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = __fdiv_rn(y[i], s);
+  }
 }
 
 // ================================================================ RMS norm -> FP8
@@ -145,23 +166,31 @@ __global__ void __launch_bounds__(kNormMaxThreads) rmsnorm_fp8_kernel(const Norm
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.res_ld : nullptr;
   T* out = p.residual_out ? static_cast<T*>(p.residual_out) + row * p.out_ld : nullptr;
+  // All loads of a thread before its first store: a store to residual_out may
+  // alias what is still to be loaded as far as the compiler knows.
+  Vec8<T> v[kIters], r[kIters];
+#pragma unroll
+  for (int it = 0; it < kIters; ++it) {
+    const int c = (it * blockDim.x + threadIdx.x) * 8;
+    if (c < p.cols) {
+      v[it] = load8<kWide>(x + c, p.cols - c);
+      if (res) r[it] = load8<kWide>(res + c, p.cols - c);
+    }
+  }
   float h[kIters][8];
   float sum = 0.f;
 #pragma unroll
   for (int it = 0; it < kIters; ++it) {
     const int c = (it * blockDim.x + threadIdx.x) * 8;
-    const int valid = p.cols - c;
-    if (valid > 0) {
-      Vec8<T> v = load8<kWide>(x + c, valid);
+    if (c < p.cols) {
       if (res) {
-        const Vec8<T> r = load8<kWide>(res + c, valid);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.e[i] = from_f32<T>(to_f32(v.e[i]) + to_f32(r.e[i]));
+        for (int i = 0; i < 8; ++i) v[it].e[i] = from_f32<T>(to_f32(v[it].e[i]) + to_f32(r[it].e[i]));
       }
-      if (out) store8<kWide>(out + c, v, valid);
+      if (out) store8<kWide>(out + c, v[it], p.cols - c);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        h[it][i] = to_f32(v.e[i]);
+        h[it][i] = to_f32(v[it].e[i]);
         sum = __fmaf_rn(h[it][i], h[it][i], sum);
       }
     } else {
@@ -205,7 +234,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) rmsnorm_fp8_kernel(const Norm
     if (valid > 0) {
       const float s = amax == 0.f ? 1.f : __fdiv_rn(amax, kE4m3Max);
       if (vec % 16 == 0) p.scales[(vec / 16) * p.s_ld + row] = s;
-      const Divider div = divider(s);
+      divide(h[it], s, amax);
       union {
         uint8_t b[8];
         __nv_fp8x2_storage_t h2[4];
@@ -213,7 +242,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) rmsnorm_fp8_kernel(const Norm
       } o;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        o.h2[i] = __nv_cvt_float2_to_fp8x2(make_float2(div(h[it][2 * i]), div(h[it][2 * i + 1])), __NV_SATFINITE, __NV_E4M3);
+        o.h2[i] = __nv_cvt_float2_to_fp8x2(make_float2(h[it][2 * i], h[it][2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
       uint8_t* q = p.q + row * p.q_ld + c;
       if constexpr (kWide) {
         *reinterpret_cast<uint2*>(q) = o.q;
@@ -228,7 +257,8 @@ __global__ void __launch_bounds__(kNormMaxThreads) rmsnorm_fp8_kernel(const Norm
 
 // ================================================================ 4-bit formats
 struct Fp4Params {
-  int64_t rows, rows_pad;  // rows_pad: rows of whole 128-row atoms
+  int64_t rows;
+  uint32_t total;          // threads: rows of whole 128-row atoms x 16 columns
   int32_t cols, atoms_k;   // atoms along K
   int64_t x_ld, v_ld;
   const void* x;
@@ -260,11 +290,46 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* y) {
   return mag | (w & (mag + 0x77777777u) & 0x88888888u);
 }
 
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-  // (1 + m / 2) 2^(e - 1), and m / 2 where e is 0.
-  const uint32_t e = (code >> 1) & 3u, m = code & 1u;
-  const float mag = e == 0 ? 0.5f * m : __uint_as_float((126u + e) << 23 | m << 22);
-  return (code & 8u) ? -mag : mag;
+// The values of 8 codes (element i in nibble i), by way of FP16, which holds them exactly.
+__device__ __forceinline__ void e2m1x8_values(uint32_t w, float* v) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// max |e| of 8 elements; a NaN wins. The 16-bit types compare two at a time.
+template <typename T>
+__device__ __forceinline__ float absmax8(const Vec8<T>& v) {
+  if constexpr (sizeof(T) == 4) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v.e[i]));
+    return m;
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(v.q);
+    uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __half>)
+        asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
+      else
+        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
+    }
+    const T* e = reinterpret_cast<const T*>(&m);
+    return max_nan(to_f32(e[0]), to_f32(e[1]));
+  }
 }
 
 __device__ __forceinline__ float found_scale(const float* partial, int n) {
@@ -294,8 +359,7 @@ __global__ void __launch_bounds__(kFp4Threads) absmax_kernel(const Fp4Params p, 
     const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
     for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
       const Vec8<T> e = load8<kWide>(x + v * 8, p.cols - v * 8);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(fabsf(to_f32(e.e[i]))));
+      m = max(m, __float_as_uint(fabsf(absmax8(e))));  // a NaN's sign must not count
     }
   }
   m = __reduce_max_sync(0xffffffffu, m);
@@ -322,69 +386,71 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quant_kernel(const Fp4Params 
     }
   }
   constexpr int kLanes = kMx ? 8 : 4;  // threads of one row's part of an atom
-  const int per_row = p.atoms_k * kLanes;
-  const int64_t total = p.rows_pad * per_row;
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * kFp4Threads + threadIdx.x;
-  const bool live = idx < total;
-  const int64_t row = live ? idx / per_row : 0;
-  const int part = live ? static_cast<int>(idx - row * per_row) : 0;
+  const uint32_t per_row = static_cast<uint32_t>(p.atoms_k) * kLanes;
+  // With a scale found by the launch before, the tensor is read a second time:
+  // from its end, which is what L2 still holds of the first reading.
+  const uint32_t block = p.partial_max ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const uint32_t idx = block * kFp4Threads + threadIdx.x;
+  const bool live = idx < p.total;
+  const uint32_t row32 = live ? idx / per_row : 0;
+  const int64_t row = row32;
+  const int part = live ? static_cast<int>(idx - row32 * per_row) : 0;
   const int c = part * 16;
   const bool has = live && row < p.rows && c < p.cols;  // cols % 32 == 0: all or none
   float v[16];
   float amax = 0.f;
   if (has) {
     const T* x = static_cast<const T*>(p.x) + row * p.x_ld + c;
+    Vec8<T> e[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) e[j] = load8<kWide>(x + 8 * j, 8);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const Vec8<T> e = load8<kWide>(x + 8 * j, 8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[8 * j + i] = to_f32(e.e[i]);
-        amax = max_nan(amax, fabsf(v[8 * j + i]));
-      }
+      for (int i = 0; i < 8; ++i) v[8 * j + i] = to_f32(e[j].e[i]);
     }
+    amax = max_nan(absmax8(e[0]), absmax8(e[1]));
   }
   if constexpr (kMx) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   uint32_t byte = 0;
   if (has) {
-    float y[16], unit;
+    float unit;
     bool zero = false;
     if constexpr (kMx) {
       // Exponent byte of 2^(floor(log2 amax) - 2): amax's own biased exponent
       // less 2 (a subnormal amax and 0 give 0, as does all below 2^-124); an
       // infinite or NaN block has scale NaN.
-      const uint32_t bits = __float_as_uint(amax);
-      const int e = static_cast<int>(bits >> 23);
+      const int e = static_cast<int>((__float_as_uint(amax) >> 23) & 0xffu);
       byte = e == 255 ? 255u : static_cast<uint32_t>(max(e - 2, 0));
       zero = byte == 255u;
       // 2^(127 - byte): exact, so y = x / b exactly. byte <= 252 here.
       const float inv = __uint_as_float((254u - min(byte, 253u)) << 23);
       unit = byte == 255u ? __uint_as_float(0x7fc00000u) : byte ? __uint_as_float(byte << 23) : 0x1p-127f;
+      const F2 inv2 = pack2(inv, inv);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] = zero ? 0.f : v[i] * inv;
+      for (int i = 0; i < 16; i += 2) unpack2(mul2(pack2(v[i], v[i + 1]), inv2), v[i], v[i + 1]);
     } else {
       const float want = __fdiv_rn(__fdiv_rn(amax, kE2m1Max), g);
       byte = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3) & 0x7fu;  // a NaN's sign is dropped
       unit = __half2float(__half(__nv_cvt_fp8_to_halfraw(byte, __NV_E4M3)));
       const float d = unit * g;
       zero = !(d > 0.f);  // an empty block, one below the scales' range, or NaN
-      const Divider div = divider(zero ? 1.f : d);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] = zero ? 0.f : div(v[i]);
+      divide(v, zero ? 1.f : d, amax);
     }
-    uint2 codes = make_uint2(e2m1x8(y), e2m1x8(y + 8));
+    const uint2 codes = zero ? make_uint2(0u, 0u) : make_uint2(e2m1x8(v), e2m1x8(v + 8));
     *reinterpret_cast<uint2*>(p.data + row * (p.cols / 2) + c / 2) = codes;
     if (p.values) {
       T* out = static_cast<T*>(p.values) + row * p.v_ld + c;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t w = j ? codes.y : codes.x;
+        float q[8];
+        e2m1x8_values(j ? codes.y : codes.x, q);
         Vec8<T> o;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float q = e2m1_value((w >> (4 * i)) & 15u) * unit;
-          if constexpr (!kMx) q *= g;
-          o.e[i] = from_f32<T>(q);
+          q[i] *= unit;
+          if constexpr (!kMx) q[i] *= g;
+          o.e[i] = from_f32<T>(q[i]);
         }
         store8<kWide>(out + 8 * j, o, 8);
       }
@@ -463,8 +529,7 @@ cudaError_t launch_fp4(const bb_quant_plan& pl) {
     const cudaError_t e = launch(absmax_kernel<T, kWide>, pl.partials, kFp4Threads, pl.stream, pl.fp, pl.partial);
     if (e != cudaSuccess) return e;
   }
-  const int64_t total = pl.fp.rows_pad * pl.fp.atoms_k * (mx ? 8 : 4);
-  const unsigned grid = static_cast<unsigned>((total + kFp4Threads - 1) / kFp4Threads);
+  const unsigned grid = (pl.fp.total + kFp4Threads - 1) / kFp4Threads;
   return mx ? launch(fp4_quant_kernel<T, true, kWide>, grid, kFp4Threads, pl.stream, pl.fp)
             : launch(fp4_quant_kernel<T, false, kWide>, grid, kFp4Threads, pl.stream, pl.fp);
 }
@@ -524,7 +589,8 @@ BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, cons
     }
     const int64_t atom_k = format == BB_LOWP_MXFP4 ? 128 : 64;
     const int64_t atoms_k = (cols + atom_k - 1) / atom_k, rows_pad = (rows + 127) / 128 * 128;
-    if (rows_pad * atoms_k * (format == BB_LOWP_MXFP4 ? 8 : 4) / kFp4Threads >= (int64_t(1) << 31) - 1) {
+    const int64_t total = rows_pad * atoms_k * (format == BB_LOWP_MXFP4 ? 8 : 4);
+    if (total > 0xffffffffll - kFp4Threads) {
       set_error("bb_fp4_quant_plan_create: %lld x %lld is more than one launch covers", (long long)rows, (long long)cols);
       return BB_ERR_ARGUMENT;
     }
@@ -543,7 +609,7 @@ BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, cons
     h->wide = aligned16(x, rows > 1 ? x_ld : 0, size) && (!values || aligned16(values, rows > 1 ? values_ld : 0, size));
     Fp4Params& p = h->fp;
     p.rows = rows;
-    p.rows_pad = rows_pad;
+    p.total = static_cast<uint32_t>(total);
     p.cols = static_cast<int32_t>(cols);
     p.atoms_k = static_cast<int32_t>(atoms_k);
     p.x_ld = x_ld;
