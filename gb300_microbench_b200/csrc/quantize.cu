@@ -52,43 +52,42 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// 8 consecutive elements. kWide: one or two 16-byte accesses (the host
-// checked base and row stride, and cols % 8 == 0, so a vector is whole);
-// otherwise element by element, elements from `valid` on read as 0 / are not written.
+// A thread's unit of columns: 32 bytes, moved by one 256-bit access.
 template <typename T>
-union alignas(16) Vec8 {
-  T e[8];
-  uint4 q[sizeof(T) * 8 / 16];
+constexpr int kVE = 32 / sizeof(T);
+template <typename T>
+union alignas(32) Vec {
+  T e[kVE<T>];
+  uint32_t w[8];
 };
 
-template <bool kWide, typename T>
-__device__ __forceinline__ Vec8<T> load8(const T* p, int valid) {
-  Vec8<T> v;
-  if constexpr (kWide) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v.q[i] = reinterpret_cast<const uint4*>(p)[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v.e[i] = i < valid ? p[i] : from_f32<T>(0.f);
-  }
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* p) {
+  Vec<T> v;
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+               : "l"(p)
+               : "memory");
   return v;
 }
-template <bool kWide, typename T>
-__device__ __forceinline__ void store8(T* p, const Vec8<T>& v, int valid) {
-  if constexpr (kWide) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = v.q[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < valid) p[i] = v.e[i];
-  }
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T>& v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]),
+               "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+               : "memory");
 }
 
 // max that keeps a NaN of either side (fmaxf drops it).
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// max(|a|, |b|, c), NaN if any is.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -151,14 +150,48 @@ struct NormParams {
   int32_t weight_f32;
 };
 
-constexpr int kNormMaxThreads = 1024;
-constexpr int kNormMaxIters = 8;  // 8 vectors of 8 columns per thread: 65536 columns
+constexpr int64_t kNormMaxCols = 65536;
 
-// One CTA per row; thread t owns the 8-column vectors t, t + blockDim, ...,
-// which stay in registers between the sum and the output (x and r are read
-// once). The 16 vectors of a scale group sit in 16 neighbouring lanes.
-template <typename T, int kIters, bool kWide>
-__global__ void __launch_bounds__(kNormMaxThreads) rmsnorm_fp8_kernel(const NormParams p) {
+// h = round_T(x + r) for one 32-byte vector. The 16-bit additions round the
+// exact sum once, which is what rounding the FP32 sum gives: where that is
+// inexact (exponents over 13 apart), the smaller term is far below half a step.
+template <typename T>
+__device__ __forceinline__ void add_vec(Vec<T>& v, const Vec<T>& r) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 4) v.e[i] += r.e[i];
+    else if constexpr (std::is_same_v<T, __half>) asm("add.rn.f16x2 %0, %0, %1;" : "+r"(v.w[i]) : "r"(r.w[i]));
+    else asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(v.w[i]) : "r"(r.w[i]));
+  }
+}
+
+// Elements 2 i and 2 i + 1 as FP32.
+template <typename T>
+__device__ __forceinline__ F2 pair_f32(const Vec<T>& v, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return pack2(v.e[2 * i], v.e[2 * i + 1]);
+  } else if constexpr (std::is_same_v<T, __half>) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v.w[i]));
+    return pack2(f.x, f.y);
+  } else {
+    return pack2(__uint_as_float(v.w[i] << 16), __uint_as_float(v.w[i] & 0xffff0000u));
+  }
+}
+
+// One CTA per row; a thread's kIters vectors of 32 bytes stay in registers
+// between the sum and the output, so x and r are read once. 16384 x 8192 BF16:
+// 138 us, 6.8 TB/s of the 940 MB it moves; what it took were 256-bit accesses,
+// packed FP32 and 16-bit arithmetic (at twice the instructions the issue slots
+// were 76 % busy and it took 168 us) and all loads in flight before the first store.
+//
+// kWide (rows and bases on 32 bytes, whole vectors): a vector is 32 bytes in a
+// row, 8 (FP32: 16) neighbouring lanes make a scale group. Otherwise a warp
+// takes the same columns with lane l holding columns l, l + 32, ...: every
+// access is a coalesced one of single elements, and 4 elements of each lane
+// make a group.
+template <typename T, int kIters, bool kWide, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) rmsnorm_fp8_kernel(const NormParams p) {
+  constexpr int VE = kVE<T>;
   __shared__ float warp_sum[32];
   grid_wait();
   grid_trigger();
@@ -166,91 +199,144 @@ __global__ void __launch_bounds__(kNormMaxThreads) rmsnorm_fp8_kernel(const Norm
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.res_ld : nullptr;
   T* out = p.residual_out ? static_cast<T*>(p.residual_out) + row * p.out_ld : nullptr;
-  // All loads of a thread before its first store: a store to residual_out may
-  // alias what is still to be loaded as far as the compiler knows.
-  Vec8<T> v[kIters], r[kIters];
-#pragma unroll
-  for (int it = 0; it < kIters; ++it) {
-    const int c = (it * blockDim.x + threadIdx.x) * 8;
-    if (c < p.cols) {
-      v[it] = load8<kWide>(x + c, p.cols - c);
-      if (res) r[it] = load8<kWide>(res + c, p.cols - c);
-    }
-  }
-  float h[kIters][8];
-  float sum = 0.f;
-#pragma unroll
-  for (int it = 0; it < kIters; ++it) {
-    const int c = (it * blockDim.x + threadIdx.x) * 8;
-    if (c < p.cols) {
-      if (res) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[it].e[i] = from_f32<T>(to_f32(v[it].e[i]) + to_f32(r[it].e[i]));
-      }
-      if (out) store8<kWide>(out + c, v[it], p.cols - c);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        h[it][i] = to_f32(v[it].e[i]);
-        sum = __fmaf_rn(h[it][i], h[it][i], sum);
-      }
+  const int lane = threadIdx.x % 32;
+  // First column of a vector, and the column of its element i.
+  auto first = [&](int it) {
+    const int unit = it * blockDim.x + threadIdx.x;
+    return kWide ? unit * VE : (unit - lane) * VE + lane;
+  };
+  auto load = [&](const T* from, int c) {
+    Vec<T> v;
+    if constexpr (kWide) {
+      v = load_vec(from + c);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[it][i] = 0.f;
+      for (int i = 0; i < VE; ++i) v.e[i] = c + 32 * i < p.cols ? from[c + 32 * i] : from_f32<T>(0.f);
+    }
+    return v;
+  };
+  // All loads of a thread before its first store: a store to residual_out may
+  // alias what is still to be loaded as far as the compiler knows.
+  Vec<T> v[kIters];
+#pragma unroll
+  for (int it = 0; it < kIters; ++it) {
+    const int c = first(it);
+    if (c < p.cols) v[it] = load(x, c);
+  }
+  if (res) {
+    Vec<T> r[kIters];
+#pragma unroll
+    for (int it = 0; it < kIters; ++it) {
+      const int c = first(it);
+      if (c < p.cols) r[it] = load(res, c);
+    }
+#pragma unroll
+    for (int it = 0; it < kIters; ++it) add_vec(v[it], r[it]);
+  }
+  F2 sum2 = pack2(0.f, 0.f);
+#pragma unroll
+  for (int it = 0; it < kIters; ++it) {
+    const int c = first(it);
+    if (c < p.cols) {
+      if (out) {
+        if constexpr (kWide) {
+          store_vec(out + c, v[it]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VE; ++i)
+            if (c + 32 * i < p.cols) out[c + 32 * i] = v[it].e[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VE / 2; ++i) {
+        const F2 h = pair_f32(v[it], i);
+        sum2 = fma2(h, h, sum2);
+      }
     }
   }
+  float sum, odd;
+  unpack2(sum2, sum, odd);
+  sum += odd;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = sum;
+  if (lane == 0) warp_sum[threadIdx.x / 32] = sum;
   __syncthreads();
-  sum = threadIdx.x % 32 < blockDim.x / 32 ? warp_sum[threadIdx.x % 32] : 0.f;
+  sum = lane < blockDim.x / 32 ? warp_sum[lane] : 0.f;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   const float rstd = rsqrtf(sum / static_cast<float>(p.cols) + p.eps);
+  const F2 rstd2 = pack2(rstd, rstd);
 #pragma unroll
   for (int it = 0; it < kIters; ++it) {
-    const int vec = it * blockDim.x + threadIdx.x;
-    const int c = vec * 8;
-    const int valid = p.cols - c;
-    float amax = 0.f;
-    if (valid > 0) {
-      float w[8];
-      if (p.weight_f32) {
-        const Vec8<float> v = load8<kWide>(static_cast<const float*>(p.weight) + c, valid);
+    const int c = first(it);
+    const bool has = c < p.cols;
+    float y[VE];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = v.e[i];
+    for (int i = 0; i < VE; ++i) y[i] = 0.f;
+    if (has) {
+      if constexpr (kWide) {
+        if (p.weight_f32) {
+          const float* w = static_cast<const float*>(p.weight) + c;
+#pragma unroll
+          for (int j = 0; j < VE / 8; ++j) {
+            const Vec<float> f = load_vec(w + 8 * j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int at = 8 * j + 2 * i;
+              unpack2(mul2(mul2(pair_f32(v[it], at / 2), rstd2), pair_f32(f, i)), y[at], y[at + 1]);
+            }
+          }
+        } else {
+          const Vec<T> w = load_vec(static_cast<const T*>(p.weight) + c);
+#pragma unroll
+          for (int i = 0; i < VE / 2; ++i)
+            unpack2(mul2(mul2(pair_f32(v[it], i), rstd2), pair_f32(w, i)), y[2 * i], y[2 * i + 1]);
+        }
       } else {
-        const Vec8<T> v = load8<kWide>(static_cast<const T*>(p.weight) + c, valid);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = to_f32(v.e[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        h[it][i] = i < valid ? h[it][i] * rstd * w[i] : 0.f;
-        amax = max_nan(amax, fabsf(h[it][i]));
+        for (int i = 0; i < VE; ++i) {
+          if (c + 32 * i >= p.cols) continue;
+          const float w = p.weight_f32 ? static_cast<const float*>(p.weight)[c + 32 * i]
+                                       : to_f32(static_cast<const T*>(p.weight)[c + 32 * i]);
+          y[i] = to_f32(v[it].e[i]) * rstd * w;
+        }
       }
     }
+    // Scale groups of this thread's elements: one (wide), or one for every four elements.
+    constexpr int kGroups = kWide ? 1 : VE / 4, kPer = VE / kGroups, kLanes = kWide ? 128 / VE : 32;
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    if (valid > 0) {
+    for (int g = 0; g < kGroups; ++g) {
+      float(&yg)[kPer] = *reinterpret_cast<float(*)[kPer]>(y + g * kPer);
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPer; i += 2) amax = max_abs(yg[i], yg[i + 1], amax);
+#pragma unroll
+      for (int d = kLanes / 2; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+      const int cg = kWide ? c : c - lane + 128 * g;  // wide: anywhere in the group; else its first column
+      if (cg >= p.cols) continue;
       const float s = amax == 0.f ? 1.f : __fdiv_rn(amax, kE4m3Max);
-      if (vec % 16 == 0) p.scales[(vec / 16) * p.s_ld + row] = s;
-      divide(h[it], s, amax);
-      union {
-        uint8_t b[8];
-        __nv_fp8x2_storage_t h2[4];
-        uint2 q;
-      } o;
+      if (lane % kLanes == 0) p.scales[(cg / 128) * p.s_ld + row] = s;
+      divide(yg, s, amax);
+    }
+    if (!has) continue;
+    union {
+      __nv_fp8x2_storage_t h2[VE / 2];
+      uint8_t b[VE];
+      uint4 q4;
+      uint2 q2;
+    } o;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o.h2[i] = __nv_cvt_float2_to_fp8x2(make_float2(h[it][2 * i], h[it][2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-      uint8_t* q = p.q + row * p.q_ld + c;
-      if constexpr (kWide) {
-        *reinterpret_cast<uint2*>(q) = o.q;
-      } else {
+    for (int i = 0; i < VE / 2; ++i)
+      o.h2[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i], y[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    uint8_t* q = p.q + row * p.q_ld + c;
+    if constexpr (kWide && VE == 16) {
+      *reinterpret_cast<uint4*>(q) = o.q4;
+    } else if constexpr (kWide) {
+      *reinterpret_cast<uint2*>(q) = o.q2;
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < valid) q[i] = o.b[i];
-      }
+      for (int i = 0; i < VE; ++i)
+        if (c + 32 * i < p.cols) q[32 * i] = o.b[i];
     }
   }
 }
@@ -309,26 +395,47 @@ __device__ __forceinline__ void e2m1x8_values(uint32_t w, float* v) {
   }
 }
 
-// max |e| of 8 elements; a NaN wins. The 16-bit types compare two at a time.
+// max |e| of a vector; a NaN wins. The 16-bit types compare two at a time.
 template <typename T>
-__device__ __forceinline__ float absmax8(const Vec8<T>& v) {
+__device__ __forceinline__ float absmax(const Vec<T>& v) {
   if constexpr (sizeof(T) == 4) {
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v.e[i]));
+    for (int i = 0; i < 8; i += 2) m = max_abs(v.e[i], v.e[i + 1], m);
     return m;
   } else {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(v.q);
-    uint32_t m = w[0] & 0x7fff7fffu;
+    uint32_t m = v.w[0] & 0x7fff7fffu;
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
+    for (int i = 1; i < 8; ++i) {
       if constexpr (std::is_same_v<T, __half>)
-        asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
+        asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(v.w[i] & 0x7fff7fffu));
       else
-        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
+        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(v.w[i] & 0x7fff7fffu));
     }
     const T* e = reinterpret_cast<const T*>(&m);
-    return max_nan(to_f32(e[0]), to_f32(e[1]));
+    return max_abs(to_f32(e[0]), to_f32(e[1]), 0.f);
+  }
+}
+
+// One vector, aligned or element by element.
+template <bool kWide, typename T>
+__device__ __forceinline__ Vec<T> get(const T* p) {
+  if constexpr (kWide) {
+    return load_vec(p);
+  } else {
+    Vec<T> v;
+#pragma unroll
+    for (int i = 0; i < kVE<T>; ++i) v.e[i] = p[i];
+    return v;
+  }
+}
+template <bool kWide, typename T>
+__device__ __forceinline__ void put(T* p, const Vec<T>& v) {
+  if constexpr (kWide) {
+    store_vec(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVE<T>; ++i) p[i] = v.e[i];
   }
 }
 
@@ -353,14 +460,13 @@ __global__ void __launch_bounds__(kFp4Threads) absmax_kernel(const Fp4Params p, 
   __shared__ uint32_t warp_max[kFp4Threads / 32];
   grid_wait();
   grid_trigger();
-  const int vecs = (p.cols + 7) / 8;
+  const int vecs = p.cols / kVE<T>;  // cols % 32 == 0
   uint32_t m = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
-    for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-      const Vec8<T> e = load8<kWide>(x + v * 8, p.cols - v * 8);
-      m = max(m, __float_as_uint(fabsf(absmax8(e))));  // a NaN's sign must not count
-    }
+#pragma unroll 2
+    for (int v = threadIdx.x; v < vecs; v += blockDim.x)
+      m = max(m, __float_as_uint(absmax(get<kWide>(x + v * kVE<T>))) & 0x7fffffffu);
   }
   m = __reduce_max_sync(0xffffffffu, m);
   if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = m;
@@ -401,15 +507,16 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quant_kernel(const Fp4Params 
   float amax = 0.f;
   if (has) {
     const T* x = static_cast<const T*>(p.x) + row * p.x_ld + c;
-    Vec8<T> e[2];
+    constexpr int VE = kVE<T>;
+    Vec<T> e[16 / VE];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) e[j] = load8<kWide>(x + 8 * j, 8);
+    for (int j = 0; j < 16 / VE; ++j) e[j] = get<kWide>(x + VE * j);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 16 / VE; ++j) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[8 * j + i] = to_f32(e[j].e[i]);
+      for (int i = 0; i < VE / 2; ++i) unpack2(pair_f32(e[j], i), v[VE * j + 2 * i], v[VE * j + 2 * i + 1]);
+      amax = max_nan(amax, absmax(e[j]));
     }
-    amax = max_nan(absmax8(e[0]), absmax8(e[1]));
   }
   if constexpr (kMx) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   uint32_t byte = 0;
@@ -441,18 +548,20 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quant_kernel(const Fp4Params 
     *reinterpret_cast<uint2*>(p.data + row * (p.cols / 2) + c / 2) = codes;
     if (p.values) {
       T* out = static_cast<T*>(p.values) + row * p.v_ld + c;
+      constexpr int VE = kVE<T>;
+      float q[16];
+      e2m1x8_values(codes.x, q);
+      e2m1x8_values(codes.y, q + 8);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float q[8];
-        e2m1x8_values(j ? codes.y : codes.x, q);
-        Vec8<T> o;
+      for (int j = 0; j < 16 / VE; ++j) {
+        Vec<T> o;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          q[i] *= unit;
-          if constexpr (!kMx) q[i] *= g;
-          o.e[i] = from_f32<T>(q[i]);
+        for (int i = 0; i < VE; ++i) {
+          float f = q[VE * j + i] * unit;
+          if constexpr (!kMx) f *= g;
+          o.e[i] = from_f32<T>(f);
         }
-        store8<kWide>(out + 8 * j, o, 8);
+        put<kWide>(out + VE * j, o);
       }
     }
   }
@@ -482,7 +591,7 @@ struct bb_quant_plan {
   cudaStream_t stream = nullptr;
   NormParams np{};
   Fp4Params fp{};
-  int threads = 0, iters = 0;
+  int threads = 0, iters = 0;  // RMS norm: vectors per thread, 0 for the widest rows
   float* partial = nullptr;  // maxima of the NVFP4 tensor scale
   int partials = 0;
   int64_t launches = 0;
@@ -492,8 +601,8 @@ namespace {
 
 size_t dtype_size(int dtype) { return dtype == BB_DTYPE_F32 ? 4 : 2; }
 bool known_dtype(int dtype) { return dtype == BB_DTYPE_BF16 || dtype == BB_DTYPE_F32 || dtype == BB_DTYPE_F16; }
-bool aligned16(const void* p, int64_t ld, size_t size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (static_cast<size_t>(ld) * size) % 16 == 0;
+bool aligned(const void* p, int64_t ld, size_t size, size_t to) {
+  return reinterpret_cast<uintptr_t>(p) % to == 0 && (static_cast<size_t>(ld) * size) % to == 0;
 }
 
 // Every launch may start before the one before it has ended (the kernels wait).
@@ -515,10 +624,10 @@ template <typename T, bool kWide>
 cudaError_t launch_norm(const bb_quant_plan& pl) {
   const unsigned grid = static_cast<unsigned>(pl.np.rows);
   switch (pl.iters) {
-    case 1: return launch(rmsnorm_fp8_kernel<T, 1, kWide>, grid, pl.threads, pl.stream, pl.np);
-    case 2: return launch(rmsnorm_fp8_kernel<T, 2, kWide>, grid, pl.threads, pl.stream, pl.np);
-    case 4: return launch(rmsnorm_fp8_kernel<T, 4, kWide>, grid, pl.threads, pl.stream, pl.np);
-    default: return launch(rmsnorm_fp8_kernel<T, 8, kWide>, grid, pl.threads, pl.stream, pl.np);
+    case 1: return launch(rmsnorm_fp8_kernel<T, 1, kWide, 512>, grid, pl.threads, pl.stream, pl.np);
+    case 2: return launch(rmsnorm_fp8_kernel<T, 2, kWide, 512>, grid, pl.threads, pl.stream, pl.np);
+    case 4: return launch(rmsnorm_fp8_kernel<T, 4, kWide, 512>, grid, pl.threads, pl.stream, pl.np);
+    default: return launch(rmsnorm_fp8_kernel<T, 64 / kVE<T>, kWide, 1024>, grid, pl.threads, pl.stream, pl.np);
   }
 }
 
@@ -606,7 +715,7 @@ BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, cons
     h->dtype = x_dtype;
     h->fmt = format;
     h->stream = static_cast<cudaStream_t>(stream);
-    h->wide = aligned16(x, rows > 1 ? x_ld : 0, size) && (!values || aligned16(values, rows > 1 ? values_ld : 0, size));
+    h->wide = aligned(x, rows > 1 ? x_ld : 0, size, 32) && (!values || aligned(values, rows > 1 ? values_ld : 0, size, 32));
     Fp4Params& p = h->fp;
     p.rows = rows;
     p.total = static_cast<uint32_t>(total);
@@ -655,10 +764,9 @@ BB_API int bb_rmsnorm_fp8_plan_create(int64_t rows, int64_t cols, const void* x,
       set_error("bb_rmsnorm_fp8_plan_create: unknown dtype %d, or a weight of dtype %d beside it", x_dtype, weight_dtype);
       return BB_ERR_ARGUMENT;
     }
-    constexpr int64_t kMaxCols = int64_t(8) * kNormMaxThreads * kNormMaxIters;
-    if (rows < 0 || rows > (int64_t(1) << 30) || cols <= 0 || cols > kMaxCols) {
+    if (rows < 0 || rows > (int64_t(1) << 30) || cols <= 0 || cols > kNormMaxCols) {
       set_error("bb_rmsnorm_fp8_plan_create: rows=%lld must lie in [0, 2^30], cols=%lld in [1, %lld]", (long long)rows,
-                (long long)cols, (long long)kMaxCols);
+                (long long)cols, (long long)kNormMaxCols);
       return BB_ERR_ARGUMENT;
     }
     if (rows > 0 && (!x || !weight || !q || !scales)) {
@@ -693,15 +801,20 @@ BB_API int bb_rmsnorm_fp8_plan_create(int64_t rows, int64_t cols, const void* x,
     h->device = dev.device;
     h->dtype = x_dtype;
     h->stream = static_cast<cudaStream_t>(stream);
-    auto wide = [&](const void* ptr, int64_t ld, size_t sz) { return aligned16(ptr, rows > 1 ? ld : 0, sz); };
-    h->wide = cols % 8 == 0 && wide(x, x_ld, size) && (!residual || wide(residual, residual_ld, size)) &&
-              (!residual_out || wide(residual_out, residual_out_ld, size)) && wide(weight, 0, wsize) &&
-              reinterpret_cast<uintptr_t>(q) % 8 == 0 && (rows <= 1 || q_ld % 8 == 0);
-    const int64_t vecs = (cols + 7) / 8;
-    h->iters = 1;
-    while (vecs > int64_t(256) * h->iters && h->iters < 4) h->iters *= 2;
-    if (vecs > int64_t(kNormMaxThreads) * h->iters) h->iters = kNormMaxIters;
-    h->threads = static_cast<int>(((vecs + h->iters - 1) / h->iters + 31) / 32 * 32);
+    auto wide = [&](const void* ptr, int64_t ld, size_t sz, size_t to) { return aligned(ptr, rows > 1 ? ld : 0, sz, to); };
+    const int64_t ve = 32 / size;
+    h->wide = cols % ve == 0 && wide(x, x_ld, size, 32) && (!residual || wide(residual, residual_ld, size, 32)) &&
+              (!residual_out || wide(residual_out, residual_out_ld, size, 32)) && wide(weight, 0, wsize, 32) &&
+              wide(q, q_ld, 1, ve);
+    // One vector per thread as far as 512 threads go, then two, four; the
+    // widest rows with 1024 threads. More vectors per thread were slower at
+    // every size (BF16: 1 x 4096 1.9 / 2.4 / 3.7 us with one / two / four,
+    // 16384 x 8192 137.9 / 139.3 / 141.8 us).
+    const int64_t vecs = (cols + ve - 1) / ve;
+    const int64_t widest = 64 / ve;
+    const int64_t per = vecs <= 512 ? 1 : vecs <= 1024 ? 2 : vecs <= 2048 ? 4 : widest;
+    h->iters = vecs <= 2048 ? static_cast<int>(per) : 0;
+    h->threads = static_cast<int>(((vecs + per - 1) / per + 31) / 32 * 32);
     NormParams& p = h->np;
     p.rows = rows;
     p.cols = static_cast<int32_t>(cols);
