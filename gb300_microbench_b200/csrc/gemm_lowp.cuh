@@ -743,7 +743,10 @@ __global__ void __launch_bounds__(Cfg<kKind, kCG>::THREADS, 1)
         float sa_next[kAhead];
         if constexpr (kGroup) {
 #pragma unroll
-          for (int j = 0; j < kAhead; ++j) sa_next[j] = j < p.k_stages ? __ldg(sa_lane + j * p.sfa_ld) : 0.f;
+          for (int j = 0; j < kAhead; ++j) {
+            sa_next[j] = j < p.k_stages ? __ldg(sa_lane) : 0.f;
+            sa_lane += p.sfa_ld;
+          }
         }
         const float* sb_row = sb + static_cast<int64_t>(nb) * p.k_stages;
         float acc[C::WARP_COLS];
@@ -777,7 +780,8 @@ __global__ void __launch_bounds__(Cfg<kKind, kCG>::THREADS, 1)
             s *= sa_next[0];
 #pragma unroll
             for (int j = 0; j + 1 < kAhead; ++j) sa_next[j] = sa_next[j + 1];
-            if (ks + kAhead < p.k_stages) sa_next[kAhead - 1] = __ldg(sa_lane + (ks + kAhead) * p.sfa_ld);
+            if (ks + kAhead < p.k_stages) sa_next[kAhead - 1] = __ldg(sa_lane);
+            sa_lane += p.sfa_ld;
           }
           const uint32_t buf = acc_iter % C::FP8_BUFS;
           // K block acc_iter's partial is complete when the MMA's commit

@@ -13,64 +13,81 @@ namespace linear {
 
 using namespace lowp;
 
+constexpr int kMaxSplits = 8;  // the portable cluster size
+
 // ---------------------------------------------------------------- few rows
 // D^T = W * X^T: the weights' rows are the tensor core's M = 128 (all of them
 // useful), the TN tokens its N (16 upwards), so one token costs the same weight
 // stream as sixteen and no arithmetic unit decodes a weight. A CTA streams
-// 128 weight rows over one share of K; the `splits` CTAs of a cluster share K
-// and add their FP32 partial sums over distributed shared memory, in rank
-// order (the result does not depend on timing).
+// 128 weight rows over one share of K. The `splits` CTAs of a cluster share K;
+// each owns some of the weight rows and adds all CTAs' FP32 partial sums of
+// them, taken over distributed shared memory, in rank order: the result does
+// not depend on timing. Up to 32 tokens the sums are sent (asynchronous stores
+// that signal the owner's barrier: one way across the cluster, 2.4 us for the
+// smallest launch against 3.2 with reading); more tokens are left in shared
+// memory and read (each asynchronous store of 4 bytes updates the barrier:
+// MXFP4 200 x 5000 x 2880 in 3 splits 15.5 us sent, 9.6 us read).
 //
 // FP8: the K blocks' FP32 scales are applied as in the tile kernel, each
-// block accumulated alone in one of kBufs TMEM buffers and promoted by the
-// epilogue warps: acc[c] += part[c] * sa[token c][kb] * sb[kb].
+// block accumulated alone in one of BUFS TMEM buffers and promoted by the
+// epilogue warps: acc[c] += part[c] * sb[kb] * sa[token c][kb].
 //
-// Bound by DRAM at one CTA pair per SM: two CTAs of up to 113 KiB share an SM
-// (TN <= 128), so about 200 KiB of weights per SM are in flight.
+// What bounds it is the weight stream, and then the ends of the launch: two
+// CTAs of up to 113 KiB share an SM (TN <= 128), so about 200 KiB of weights
+// per SM are in flight, and CTAs of the next launch start beside the last
+// ones of this, set up, and fetch their first weights into L2.
 template <int kKind, int kTN>
 struct FewCfg {
   static constexpr int TN = kTN;
   static constexpr bool FP4 = is_fp4(kKind);
-  static constexpr int CTAS_PER_SM = TN <= 128 ? 2 : 1;
+  static constexpr int CTAS_PER_SM = FP4 || TN <= 64 ? 2 : 1;  // FP8's 64 accumulators a thread want a whole SM's registers
   static constexpr int EPI_W = TN <= 32 ? 4 : 8;  // epilogue warps: lane quarters x column halves
   static constexpr int THREADS = 64 + 32 * EPI_W;
   static constexpr int COLS = TN * 4 / EPI_W;     // accumulator columns per epilogue thread
-  static constexpr int K_PER_STAGE = FP4 ? 256 : 128;
+  static constexpr int CHUNK = COLS == 32 ? 32 : 16;  // columns of one TMEM load
   static constexpr int MMAS = 4;
   static constexpr int ATOMS = kKind == kNvfp4 ? 4 : kKind == kMxfp4 ? 2 : 0;
-  static constexpr int X_BLOCKS = TN > 128 ? 2 : 1;  // 128-row scale blocks of the tokens
   static constexpr int W_BYTES = 128 * ROW_BYTES;
   static constexpr int X_BYTES = TN * ROW_BYTES;
-  static constexpr int SFW_BYTES = ATOMS * SF_ATOM;
-  static constexpr int SFX_BYTES = X_BLOCKS * ATOMS * SF_ATOM;
-  static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + SFW_BYTES + SFX_BYTES;
-  static constexpr int SCALE_BYTES = FP4 ? 0 : EPI_W * COLS * 4;  // FP8: a K block's scales, per epilogue warp
-  static constexpr int TAIL_BYTES = SCALE_BYTES + BAR_BYTES;
+  static constexpr int SF_BYTES = ATOMS * SF_ATOM;  // of the weights, and as much of the tokens
+  static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + 2 * SF_BYTES;
+  // Partial sums. Sent: [split][token][owned row] (splits * owned rows are 128
+  // and a few) in a place of their own. Read: [token][128 rows] over the ring.
+  static constexpr bool SEND = TN <= 32;
+  static constexpr int SEND_BYTES = SEND ? TN * (128 + kMaxSplits) * 4 : 0;
+  // FP8: every epilogue warp keeps the scales of SCALE_SLOTS K blocks (its
+  // tokens' and, behind them, the weights').
+  static constexpr int SCALE_SLOTS = 4;
+  static constexpr int SCALE_PITCH = COLS + 4;
+  static constexpr int SCALE_BYTES = FP4 ? 0 : EPI_W * SCALE_SLOTS * SCALE_PITCH * 4;
+  static constexpr int TAIL_BYTES = SEND_BYTES + SCALE_BYTES + BAR_BYTES;
   static constexpr int LIMIT = CTAS_PER_SM == 2 ? 115712 : SMEM_LIMIT;
   static constexpr int STAGES_FIT = (LIMIT - 1024 - TAIL_BYTES) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_FIT < 8 ? STAGES_FIT : 8;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TAIL_BYTES;
   // FP8: partial buffers. FP4: one accumulator, then the scale columns.
-  static constexpr int BUFS = FP4 ? 1 : TN <= 32 ? 4 : 2;
+  static constexpr int BUFS = FP4 ? 1 : TN == 16 ? 4 : TN == 32 ? 3 : 2;
   static constexpr int SF_COL = TN;
-  static constexpr int SF_COLS = ATOMS * 4 * (1 + X_BLOCKS);
+  static constexpr int SF_COLS = ATOMS * 8;
   static constexpr int COLS_USED = FP4 ? TN + SF_COLS : BUFS * TN;
-  static constexpr int TMEM = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
-  static_assert(TMEM * CTAS_PER_SM <= 512, "TMEM of the CTAs that share an SM");
+  static constexpr int TMEM = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : 256;
+  static_assert(COLS_USED <= 256 && TMEM * CTAS_PER_SM <= 512, "TMEM of the CTAs that share an SM");
   static_assert(STAGES >= 3 && SMEM_BYTES <= LIMIT, "shared memory");
-  static_assert(TN * 128 * 4 <= STAGES * STAGE_BYTES, "partial sums fit the ring");
-  static_assert((2 * STAGES + 2 * BUFS + 3) * 8 <= BAR_BYTES, "barrier area");
+  static_assert(SEND || TN * 512 <= STAGES * STAGE_BYTES, "partial sums fit the ring");
+  static_assert((2 * STAGES + BUFS + 3) * 8 <= BAR_BYTES, "barrier area");
   static_assert(BUFS < STAGES, "a stage's barrier tells the epilogue of its block");
 };
 
-constexpr int kMaxSplits = 8;  // the portable cluster size
+// Weights fetched into L2 ahead of the wait (NVFP4 1 x 8192 x 8192: none 9.7 us,
+// three stages 8.9, six 9.3; FP8 1 x 14336 x 4096: 13.5, 13.1, 13.3).
+constexpr int kPrefetchStages = 3;
 
 struct FewParams {
   int32_t m, n;
-  int32_t k_stages, splits;
-  int32_t kb;          // FP8: K blocks
-  const float* sfa;    // FP8: [kb][sfa_ld]
-  const float* sfb;    // FP8: [n blocks][kb]
+  int32_t k_stages, splits, tiles_n;
+  int32_t owned;       // weight rows a CTA of the cluster owns: rank r has [r * owned, + owned) of the 128
+  const float* sfa;    // FP8: [K block][sfa_ld]
+  const float* sfb;    // FP8: [weight row block][K block]
   int64_t sfa_ld, ldd;
   float scale;
   const float* scale_dev[2];
@@ -85,14 +102,36 @@ __device__ __forceinline__ void store_one(void* d, int dtype, int64_t at, float 
   else static_cast<float*>(d)[at] = v;
 }
 
-// N columns of this warp's 32 TMEM lanes.
+// `count` of N tokens of one column of D.
 template <int N>
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t* r) {
-  if constexpr (N >= 32) {
+__device__ __forceinline__ void store_tokens(const FewParams& p, int token, int count, int n, const float (&v)[N], float s) {
+  if (n >= p.n) return;
+  const int64_t at = token * p.ldd + n;
+  if (p.d_dtype == BB_DTYPE_BF16) {
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.d) + at;
 #pragma unroll
-    for (int c = 0; c < N / 32; ++c) tmem_ld_32x32b_x32(taddr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
+    for (int c = 0; c < N; ++c)
+      if (c < count) d[c * p.ldd] = __float2bfloat16_rn(v[c] * s);
+  } else if (p.d_dtype == BB_DTYPE_F16) {
+    __half* d = static_cast<__half*>(p.d) + at;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if (c < count) d[c * p.ldd] = __float2half_rn(v[c] * s);
   } else {
-    static_assert(N == 16, "16 or a multiple of 32");
+    float* d = static_cast<float*>(p.d) + at;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if (c < count) d[c * p.ldd] = v[c] * s;
+  }
+}
+
+// 16 or 32 columns of this warp's 32 TMEM lanes.
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[N]) {
+  static_assert(N == 16 || N == 32, "16 or 32 columns");
+  if constexpr (N == 32) {
+    tmem_ld_32x32b_x32(taddr, r);
+  } else {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -100,6 +139,19 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t* r) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
   }
+}
+
+// 4 bytes into shared memory, zero where `valid` is false (nothing is read then).
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+
+// 4 bytes into a CTA of the cluster (shared::cluster addresses), counted by a
+// barrier of that CTA.
+__device__ __forceinline__ void st_async_f32(uint32_t addr, float v, uint32_t mbar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)),
+               "r"(mbar)
+               : "memory");
 }
 
 __device__ __forceinline__ float4 ld_cluster_v4f(uint32_t cluster_addr) {
@@ -123,20 +175,26 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
   uint8_t* smem_w = smem;
   uint8_t* smem_x = smem_w + STAGES * C::W_BYTES;
   uint8_t* smem_sfw = smem_x + STAGES * C::X_BYTES;
-  uint8_t* smem_sfx = smem_sfw + STAGES * C::SFW_BYTES;
-  float* smem_scale = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES + C::SCALE_BYTES);
+  uint8_t* smem_sfx = smem_sfw + STAGES * C::SF_BYTES;
+  uint8_t* tail = smem + STAGES * C::STAGE_BYTES;
+  float* sums = reinterpret_cast<float*>(C::SEND ? tail : smem);
+  if constexpr (C::SEND) tail += C::SEND_BYTES;
+  float* smem_scale = reinterpret_cast<float*>(tail);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tail + C::SCALE_BYTES);
   uint64_t* full = bars;
   uint64_t* empty = bars + STAGES;
   uint64_t* acc_empty = bars + 2 * STAGES;  // [BUFS], FP8
   uint64_t* done = acc_empty + C::BUFS;     // every MMA of this CTA has finished
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* received = done + 1;            // the other CTAs' partial sums are here
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(received + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int n_blk = blockIdx.x / p.splits;
+  const int unit = blockIdx.x / p.splits;  // output tile: 128 weight rows x TN tokens
+  const int m0 = unit / p.tiles_n * C::TN, n_blk = unit % p.tiles_n;
   const int ks0 = static_cast<int>(static_cast<int64_t>(p.k_stages) * rank / p.splits);
   const int ks1 = static_cast<int>(static_cast<int64_t>(p.k_stages) * (rank + 1) / p.splits);
+  const int mine = min(p.owned, 128 - rank * p.owned);  // weight rows this CTA owns
 
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tm_w);
@@ -151,39 +209,42 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
     }
     for (int b = 0; b < C::BUFS; ++b) mbar_init(smem_u32(&acc_empty[b]), C::EPI_W);
     mbar_init(smem_u32(done), 1);
+    mbar_init(smem_u32(received), 1);
     fence_mbarrier_init_cluster();
+    if (C::SEND && p.splits > 1) mbar_arrive_expect_tx(smem_u32(received), (p.splits - 1) * mine * p.m * 4);
   }
   if (warp == 1) {
     tmem_alloc<1>(smem_u32(tmem_slot), C::TMEM);
     tmem_relinquish<1>();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-
-  // All of the above overlaps the end of the kernel before. The weights may
-  // come from that kernel too, so before the wait they are fetched into L2
-  // only, where its writes land as well.
-  if (warp == 0 && elect_one()) {
-    for (int ks = ks0; ks < ks1 && ks < ks0 + STAGES; ++ks) tma_prefetch_2d(&tm_w, ks * ROW_BYTES, n_blk * 128);
+  // The weights may come from the launch before, so ahead of the wait below
+  // they are fetched into L2 only, where that launch's writes land as well.
+  if (warp == 2 && elect_one()) {
+    for (int ks = ks0; ks < ks1 && ks < ks0 + kPrefetchStages; ++ks)
+      tma_prefetch_2d(&tm_w, ks * ROW_BYTES, n_blk * 128);
   }
   __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  // `received` is ready for the other CTAs' signals; waited for before sending.
+  if (C::SEND && p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   grid_wait();
   grid_trigger();
 
-  float scale = p.scale;
-  float* red = reinterpret_cast<float*>(smem);  // [TN][128] partial sums, over the ring once it is idle
   const int q = warp & 3, half = (warp - 2) / 4;
-  const int row = q * 32 + lane;       // weight row within the block (epilogue)
-  const int col0 = half * C::COLS;     // first token of this thread (epilogue)
+  const int row = q * 32 + lane;    // weight row within the block (epilogue)
+  const int col0 = half * C::COLS;  // first token of this thread (epilogue)
   const int n = n_blk * 128 + row;
-  auto put = [&](int c, float v) {
-    if (c < p.m && n < p.n) store_one(p.d, p.d_dtype, c * p.ldd + n, v * scale);
-  };
+  const int tokens = min(C::COLS, p.m - m0 - col0);  // of this thread; may be negative
+  float scale = p.scale;
+  F2 acc[C::FP4 ? 1 : C::COLS / 2];
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + col0;
+  bool ok = true;
 
   if (warp == 0) {
-    bool ok = true;
+    // ------------------------------------------------------------ producer
     int stage = 0;
     uint32_t phase = 0;
     for (int ks = ks0; ks < ks1; ++ks) {
@@ -195,10 +256,10 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
         const uint32_t fb = smem_u32(&full[stage]);
         mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
         tma_load_2d(smem_u32(smem_w + stage * C::W_BYTES), &tm_w, fb, ks * ROW_BYTES, n_blk * 128);
-        tma_load_2d(smem_u32(smem_x + stage * C::X_BYTES), &tm_x, fb, ks * ROW_BYTES, 0);
+        tma_load_2d(smem_u32(smem_x + stage * C::X_BYTES), &tm_x, fb, ks * ROW_BYTES, m0);
         if constexpr (C::FP4) {
-          tma_load_2d(smem_u32(smem_sfw + stage * C::SFW_BYTES), &tm_sfw, fb, ks * 64 * C::ATOMS, n_blk);
-          tma_load_2d(smem_u32(smem_sfx + stage * C::SFX_BYTES), &tm_sfx, fb, ks * 64 * C::ATOMS, 0);
+          tma_load_2d(smem_u32(smem_sfw + stage * C::SF_BYTES), &tm_sfw, fb, ks * 64 * C::ATOMS, n_blk);
+          tma_load_2d(smem_u32(smem_sfx + stage * C::SF_BYTES), &tm_sfx, fb, ks * 64 * C::ATOMS, m0 / 128);
         }
       }
       __syncwarp();
@@ -220,6 +281,7 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
       bounded_sleep_ns(2000000);  // aborted: let copies already issued land
     }
   } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
     int stage = 0;
     uint32_t phase = 0, it = 0;
     const uint64_t w_desc0 = sw128_kmajor_desc(smem_u32(smem_w)), x_desc0 = sw128_kmajor_desc(smem_u32(smem_x));
@@ -239,25 +301,23 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
         const uint64_t w_desc = w_desc0 + static_cast<uint64_t>(stage) * (C::W_BYTES >> 4);
         const uint64_t x_desc = x_desc0 + static_cast<uint64_t>(stage) * (C::X_BYTES >> 4);
         if constexpr (C::FP4) {
-          const uint64_t sfw = sfw_desc0 + static_cast<uint64_t>(stage) * (C::SFW_BYTES >> 4);
-          const uint64_t sfx = sfx_desc0 + static_cast<uint64_t>(stage) * (C::SFX_BYTES >> 4);
+          const uint64_t sfw = sfw_desc0 + static_cast<uint64_t>(stage) * (C::SF_BYTES >> 4);
+          const uint64_t sfx = sfx_desc0 + static_cast<uint64_t>(stage) * (C::SF_BYTES >> 4);
           constexpr int per_atom = C::MMAS / C::ATOMS;  // instructions that share an atom
 #pragma unroll
           for (int g = 0; g < C::MMAS; ++g) {
             const int a = g / per_atom;
             const uint32_t t_w = tmem + C::SF_COL + 4 * a;
-            const uint32_t t_x = tmem + C::SF_COL + 4 * C::ATOMS + 4 * C::X_BLOCKS * a;
+            const uint32_t t_x = t_w + 4 * C::ATOMS;
             if (g % per_atom == 0) {
               tmem_cp_desc<1>(t_w, sfw + a * (SF_ATOM >> 4));
-#pragma unroll
-              for (int b = 0; b < C::X_BLOCKS; ++b)
-                tmem_cp_desc<1>(t_x + 4 * b, sfx + (b * C::ATOMS + a) * (SF_ATOM >> 4));
+              tmem_cp_desc<1>(t_x, sfx + a * (SF_ATOM >> 4));
             }
-            const uint32_t acc = (it | g) != 0 ? 1u : 0u;
+            const uint32_t accumulate = (it | g) != 0 ? 1u : 0u;
             if constexpr (kKind == kNvfp4)
-              mma_nvf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_nvf4(128, C::TN), t_w, t_x, acc);
+              mma_nvf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_nvf4(128, C::TN), t_w, t_x, accumulate);
             else
-              mma_mxf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_mxf4(128, C::TN, 2 * (g % 2)), t_w, t_x, acc);
+              mma_mxf4<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_mxf4(128, C::TN, 2 * (g % 2)), t_w, t_x, accumulate);
           }
         } else {
 #pragma unroll
@@ -277,52 +337,39 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
     __syncwarp();
     bb_wait_warp(smem_u32(done), 0, p.status, kDevTimeoutMma, /*honor_abort=*/false);
   } else {
+    // ------------------------------------------------------------ epilogue
     if (p.scale_dev[0]) scale *= *p.scale_dev[0];
     if (p.scale_dev[1]) scale *= *p.scale_dev[1];
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + col0;
-    float acc[C::COLS];
-    bool ok = true;
     if constexpr (C::FP4) {
-      ok = bb_wait_warp(smem_u32(done), 0, p.status, kDevTimeoutEpilogue);
+      ok = bb_wait_warp<false, false>(smem_u32(done), 0, p.status, kDevTimeoutEpilogue);
       tc_fence_after();
-      if (ok) {
-        tmem_ld_cols<C::COLS>(taddr, reinterpret_cast<uint32_t*>(acc));
-        tmem_ld_wait();
-      }
     } else {
+      float* my_scale = smem_scale + (warp - 2) * C::SCALE_SLOTS * C::SCALE_PITCH;
+      auto fetch_scales = [&](int ks) {
+        if (ks < ks1) {
+          const uint32_t dst = smem_u32(my_scale + (ks - ks0) % C::SCALE_SLOTS * C::SCALE_PITCH);
+          const float* src = p.sfa + ks * p.sfa_ld + m0 + col0;
 #pragma unroll
-      for (int c = 0; c < C::COLS; ++c) acc[c] = 0.f;
-      float* my_scale = smem_scale + (warp - 2) * C::COLS;  // this warp's token scales of the current K block
-      constexpr int kPer = (C::COLS + 31) / 32;
-      // The lane's token scales times the weights' scale of the next kAhead K
-      // blocks: a load takes up to 800 ns, a block of weights half of that.
-      constexpr int kAhead = 4;
-      float next[kAhead][kPer], next_b[kAhead];
-      auto load = [&](int slot, int kb) {
-        if (kb >= ks1) return;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int c = lane + 32 * j;
-          next[slot][j] = c < C::COLS && col0 + c < p.m ? __ldg(p.sfa + kb * p.sfa_ld + col0 + c) : 0.f;
+          for (int j = 0; j < (C::COLS + 31) / 32; ++j) {
+            const int c = lane + 32 * j;
+            if (c < C::COLS) cp_async_4(dst + c * 4, c < tokens ? src + c : p.sfa, c < tokens);
+          }
+          if (lane == 31) cp_async_4(dst + C::COLS * 4, p.sfb + static_cast<int64_t>(n_blk) * p.k_stages + ks, true);
         }
-        next_b[slot] = __ldg(p.sfb + static_cast<int64_t>(n_blk) * p.kb + kb);
+        cp_async_commit();
       };
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) load(j, ks0 + j);
+      for (int i = 0; i < C::SCALE_SLOTS - 1; ++i) fetch_scales(ks0 + i);
+#pragma unroll
+      for (int c = 0; c < C::COLS / 2; ++c) acc[c] = pack2(0.f, 0.f);
       for (int ks = ks0; ks < ks1; ++ks) {
         const uint32_t it = ks - ks0, buf = it % C::BUFS;
+        __syncwarp();  // the slot written next was read in the block before
+        fetch_scales(ks + C::SCALE_SLOTS - 1);
+        cp_async_wait<C::SCALE_SLOTS - 1>();
         __syncwarp();
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (lane + 32 * j < C::COLS) my_scale[lane + 32 * j] = next[0][j] * next_b[0];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i + 1 < kAhead; ++i) {
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) next[i][j] = next[i + 1][j];
-          next_b[i] = next_b[i + 1];
-        }
-        load(kAhead - 1, ks + kAhead);
+        const float* sc = my_scale + it % C::SCALE_SLOTS * C::SCALE_PITCH;
+        const F2 sb = pack2(sc[C::COLS], sc[C::COLS]);
         // The commit that releases the operand stage also says that the K
         // block's partial is complete; the MMA warp runs at most BUFS < STAGES
         // blocks ahead, so the parity cannot be overtaken.
@@ -332,52 +379,116 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
           break;
         }
         tc_fence_after();
-        constexpr int kChunk = C::COLS < 32 ? C::COLS : 32;
 #pragma unroll
-        for (int c0 = 0; c0 < C::COLS; c0 += kChunk) {
-          uint32_t r[kChunk];
-          tmem_ld_cols<kChunk>(taddr + buf * C::TN + c0, r);
+        for (int c0 = 0; c0 < C::COLS; c0 += C::CHUNK) {
+          uint32_t r[C::CHUNK];
+          tmem_ld_cols(taddr + buf * C::TN + c0, r);
           tmem_ld_wait();
-          if (c0 + kChunk == C::COLS) {
+          if (c0 + C::CHUNK == C::COLS) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&acc_empty[buf]));
           }
 #pragma unroll
-          for (int c = 0; c < kChunk; c += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(my_scale + c0 + c);
-            acc[c0 + c] = fmaf(__uint_as_float(r[c]), s.x, acc[c0 + c]);
-            acc[c0 + c + 1] = fmaf(__uint_as_float(r[c + 1]), s.y, acc[c0 + c + 1]);
-            acc[c0 + c + 2] = fmaf(__uint_as_float(r[c + 2]), s.z, acc[c0 + c + 2]);
-            acc[c0 + c + 3] = fmaf(__uint_as_float(r[c + 3]), s.w, acc[c0 + c + 3]);
+          for (int c = 0; c < C::CHUNK; c += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(sc + c0 + c);
+            F2& a0 = acc[(c0 + c) / 2];
+            F2& a1 = acc[(c0 + c) / 2 + 1];
+            a0 = fma2(mul2(pack2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sb), pack2(s.x, s.y), a0);
+            a1 = fma2(mul2(pack2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), sb), pack2(s.z, s.w), a1);
           }
         }
       }
-      if (p.splits > 1) ok = ok && bb_wait_warp(smem_u32(done), 0, p.status, kDevTimeoutEpilogue);
-    }
-    if (ok) {
-      if (p.splits == 1) {
-#pragma unroll
-        for (int c = 0; c < C::COLS; ++c) put(col0 + c, acc[c]);
-      } else {
-        // The ring is idle (`done`): no copy is in flight and every MMA has read its operands.
-#pragma unroll
-        for (int c = 0; c < C::COLS; ++c)
-          if (col0 + c < p.m) red[(col0 + c) * 128 + row] = acc[c];
-      }
+      cp_async_wait<0>();
+      if (!C::SEND && p.splits > 1)
+        ok = bb_wait_warp<false, false>(smem_u32(done), 0, p.status, kDevTimeoutEpilogue) && ok;
     }
   }
-  if (p.splits > 1) {
+  if (C::SEND && p.splits > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  if (warp >= 2) {
+    // This thread's sums, CHUNK tokens at a time: to D, to the row's owner, or
+    // into the ring, which is idle (`done`: every copy has landed and been read).
+    const int owner = row / p.owned;
+    const uint32_t at = ((rank * C::TN + col0) * p.owned + row - owner * p.owned) * 4;
+    const uint32_t to = mapa_shared(smem_u32(sums) + at, owner), to_bar = mapa_shared(smem_u32(received), owner);
+#pragma unroll
+    for (int c0 = 0; c0 < C::COLS; c0 += C::CHUNK) {
+      if (c0 >= tokens) break;
+      float v[C::CHUNK];
+      if constexpr (C::FP4) {
+        uint32_t r[C::CHUNK];
+        tmem_ld_cols(taddr + c0, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < C::CHUNK; ++c) v[c] = __uint_as_float(r[c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < C::CHUNK; c += 2) unpack2(acc[(c0 + c) / 2], v[c], v[c + 1]);
+      }
+      if (p.splits == 1) {
+        store_tokens(p, m0 + col0 + c0, min(C::CHUNK, tokens - c0), n, v, scale);
+      } else if constexpr (C::SEND) {
+#pragma unroll
+        for (int c = 0; c < C::CHUNK; ++c) {
+          if (c0 + c >= tokens) continue;
+          if (owner == rank) sums[at / 4 + (c0 + c) * p.owned] = v[c];
+          else st_async_f32(to + (c0 + c) * p.owned * 4, v[c], to_bar);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < C::CHUNK; ++c) sums[(col0 + c0 + c) * 128 + row] = v[c];
+      }
+      __syncwarp();
+    }
+  }
+  if (C::SEND && p.splits > 1) {
+    // Arrived: this CTA sends nothing more. Waited for at the end: no CTA leaves while another still sends.
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    if (warp >= 2) {
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * C::EPI_W) : "memory");  // the CTA's own sums
+      bb_wait_warp<true, false>(smem_u32(received), 0, p.status, kDevTimeoutEpilogue);
+      // Element e of the m x mine sums, e = thread, thread + threads, ...
+      constexpr int kThreads = 32 * C::EPI_W;
+      const int e0 = threadIdx.x - 64;
+      int token = e0 / mine, r0 = e0 - token * mine;
+      const int step = kThreads / mine, step_row = kThreads - step * mine;
+      while (token < p.m) {
+        const float* from = sums + token * p.owned + r0;
+        float f[kMaxSplits];
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) f[r] = r < p.splits ? from[r * C::TN * p.owned] : 0.f;
+        float v = f[0];
+#pragma unroll
+        for (int r = 1; r < kMaxSplits; ++r) v += f[r];
+        const int at_n = n_blk * 128 + rank * p.owned + r0;
+        if (at_n < p.n) store_one(p.d, p.d_dtype, token * p.ldd + at_n, v * scale);
+        token += step;
+        r0 += step_row;
+        if (r0 >= mine) {
+          r0 -= mine;
+          ++token;
+        }
+      }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  }
+  if (!C::SEND && p.splits > 1) {
     __syncwarp();
     cluster_sync();
     if (warp >= 2) {
       // Rank r adds the tokens r, r + splits, ... of all ranks' partial sums: a
       // warp per token, a lane four weight rows. Remote loads take most of a
-      // microsecond each, so those of all ranks and of kBatch tokens are in flight together.
-      constexpr int kBatch = C::TN <= 16 ? 1 : 2;
-      const uint32_t base = smem_u32(red) + lane * 16;
+      // microsecond each, so those of all ranks and of two tokens are in flight together.
+      constexpr int kBatch = 2;
+      const int count = min(C::TN, p.m - m0);
+      const uint32_t base = smem_u32(sums) + lane * 16;
       const int n4 = n_blk * 128 + lane * 4;
-      for (int c = rank + (warp - 2) * p.splits; c < p.m; c += p.splits * C::EPI_W * kBatch) {
+      for (int c = rank + (warp - 2) * p.splits; c < count; c += p.splits * C::EPI_W * kBatch) {
         float4 v[kBatch][kMaxSplits];
 #pragma unroll
         for (int r = 0; r < kMaxSplits; ++r) {
@@ -385,12 +496,12 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
           const uint32_t from = mapa_shared(base + c * 512, r);
 #pragma unroll
           for (int j = 0; j < kBatch; ++j)
-            if (c + j * p.splits * C::EPI_W < p.m) v[j][r] = ld_cluster_v4f(from + j * p.splits * C::EPI_W * 512);
+            if (c + j * p.splits * C::EPI_W < count) v[j][r] = ld_cluster_v4f(from + j * p.splits * C::EPI_W * 512);
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
           const int token = c + j * p.splits * C::EPI_W;
-          if (token >= p.m) break;
+          if (token >= count) break;
           float4 sum = v[j][0];
 #pragma unroll
           for (int r = 1; r < kMaxSplits; ++r) {
@@ -400,7 +511,7 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
             sum.z += v[j][r].z;
             sum.w += v[j][r].w;
           }
-          const int64_t at = token * p.ldd + n4;
+          const int64_t at = (m0 + token) * p.ldd + n4;
           const float out[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -491,8 +602,7 @@ int launch_few_kind(const bb_linear_plan& pl) {
     case 16: return launch_few<kKind, 16>(pl);
     case 32: return launch_few<kKind, 32>(pl);
     case 64: return launch_few<kKind, 64>(pl);
-    case 128: return launch_few<kKind, 128>(pl);
-    default: return launch_few<kKind, 256>(pl);
+    default: return launch_few<kKind, 128>(pl);
   }
 }
 
@@ -557,18 +667,27 @@ int launch_linear(const bb_linear_plan& pl) {
   return launch_kind<kFp8Group>(pl);
 }
 
+// Which kernel: the one for few rows up to 128 rows, and above as long as its
+// 128 x 128 tiles are not more than the SMs. The tile kernel's 256 x 256 pairs
+// would leave most SMs idle there (FP8, few against tiles: 256 x 4096 x 4096
+// 14.7 us / 19.8, 512 x 1024 x 8192 15.0 / 35.2, 512 x 4096 x 4096 20.5 / 20.5;
+// MXFP4 200 x 5000 x 2880 8.7 / 9.7).
+bool use_few(int64_t m, int64_t rb_n, int sm_count) { return m <= 128 || rb_n * ((m + 127) / 128) <= sm_count; }
+
 // K splits of the few-rows kernel. One CTA per SM suffices for a short K: more
 // of them only add to the exchange (MXFP4 128 x 4096 x 4096, 32 row blocks:
-// 4 splits 8.4 us, 8 splits 13.3). A second CTA per SM keeps more of a long
-// weight stream in flight (NVFP4 1 x 8192 x 8192: 2 splits 10.7 us, 4 splits
-// 9.2; FP8 1 x 14336 x 4096: 1 split 14.4, 2 splits 13.3) where each still has
+// 4 splits 8.4 us, 8 splits 12.8). A second CTA per SM keeps more of a long
+// weight stream in flight (NVFP4 1 x 8192 x 8192: 2 splits 10.8 us, 4 splits
+// 9.2; FP8 1 x 14336 x 4096: 1 split 14.6, 2 splits 13.0) where each still has
 // kLongShare stages. Never more CTAs than are resident at once: a second wave
-// costs half the kernel (5 splits of the same NVFP4 case 14.2 us).
+// costs half the kernel (5 splits of the same NVFP4 case 12.4 us). Sums of
+// many tokens are read from at most six CTAs (MXFP4 200 x 1024 x 8192: 6 splits
+// 7.8 us, 8 splits 9.1; FP8 12.4 and 18.6).
 constexpr int kLongShare = 8;
-int choose_splits(int units, int k_stages, int sm_count, int ctas_per_sm) {
-  auto within = [](int s, int most) { return s < most ? s : most; };
-  int s = within(within(sm_count / units, kMaxSplits), k_stages / 2);
-  const int more = within(within(sm_count * ctas_per_sm / units, kMaxSplits), k_stages / kLongShare);
+int choose_splits(int units, int k_stages, int sm_count, int ctas_per_sm, int most) {
+  auto within = [](int s, int limit) { return s < limit ? s : limit; };
+  int s = within(within(sm_count / units, most), k_stages / 2);
+  const int more = within(within(sm_count * ctas_per_sm / units, most), k_stages / kLongShare);
   if (more > s) s = more;
   return s < 1 ? 1 : s;
 }
@@ -586,8 +705,7 @@ void few_info(int tn, bb_lowp_info* info) {
     case 16: set(FewCfg<kKind, 16>{}); break;
     case 32: set(FewCfg<kKind, 32>{}); break;
     case 64: set(FewCfg<kKind, 64>{}); break;
-    case 128: set(FewCfg<kKind, 128>{}); break;
-    default: set(FewCfg<kKind, 256>{}); break;
+    default: set(FewCfg<kKind, 128>{}); break;
   }
 }
 
@@ -694,16 +812,17 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
     const int stage_atoms = kind == BB_LOWP_NVFP4 ? 4 : 2;
     const int64_t rb_m = (m + 127) / 128, rb_n = (n + 127) / 128;
     const int k_stages = static_cast<int>((row_bytes + ROW_BYTES - 1) / ROW_BYTES);
-    h->few = m <= 256;
+    h->few = use_few(m, rb_n, dev.sm_count);
     if (h->few) {
-      h->tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
+      h->tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
       FewParams& p = h->fp;
       p.m = static_cast<int32_t>(m);
       p.n = static_cast<int32_t>(n);
       p.k_stages = k_stages;
-      const int units = static_cast<int>(rb_n);
-      p.splits = choose_splits(units, k_stages, dev.sm_count, h->tn <= 128 ? 2 : 1);
-      p.kb = static_cast<int32_t>((k + 127) / 128);
+      const int units = static_cast<int>(rb_n * (m > h->tn ? (m + h->tn - 1) / h->tn : 1));
+      p.tiles_n = static_cast<int32_t>(rb_n);
+      p.splits = choose_splits(units, k_stages, dev.sm_count, fp8 && h->tn > 64 ? 1 : 2, h->tn > 32 ? 6 : kMaxSplits);
+      p.owned = (128 + p.splits - 1) / p.splits;
       p.sfa = static_cast<const float*>(sfa);
       p.sfb = static_cast<const float*>(sfb);
       p.sfa_ld = sfa_ld;
@@ -761,7 +880,7 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
         h->tm_sfa = h->tm_a;  // unused: FP32 scales do not travel by TMA
         h->tm_sfb = h->tm_b;
       } else {
-        if (rc == BB_OK) rc = map_atoms(&h->tm_sfa, sfa, atoms_k, rb_m, stage_atoms, h->few && h->tn > 128 ? 2 : 1);
+        if (rc == BB_OK) rc = map_atoms(&h->tm_sfa, sfa, atoms_k, rb_m, stage_atoms, 1);
         if (rc == BB_OK) rc = map_atoms(&h->tm_sfb, sfb, atoms_k, rb_n, stage_atoms, h->few ? 1 : 2);
       }
       h->tm_d = h->tm_a;

@@ -91,27 +91,6 @@ __device__ __forceinline__ float max_abs(float a, float b, float c) {
   return r;
 }
 
-// Two FP32 operations per instruction (sm_100's packed FP32).
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 pack2(float lo, float hi) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack2(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-
 // y[i] / s for the N values of a block whose magnitudes are at most `most`,
 // correctly rounded: with r = 1 / s correctly rounded, one residual step
 // q = q0 + (y - q0 s) r of q0 = y r gives the rounded quotient (Markstein, IBM

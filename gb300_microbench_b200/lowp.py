@@ -336,8 +336,11 @@ class Fp8GroupOperand:
 
     @property
     def values(self) -> torch.Tensor:
-        """The E4M3 values, (R, K) float8_e4m3fn (a view)."""
-        return self.data.view(torch.float8_e4m3fn)
+        """The E4M3 values, (R, K) float8_e4m3fn (a view of ``data``)."""
+        view = self.__dict__.get("_values")
+        if view is None or view.data_ptr() != self.data.data_ptr():
+            view = self._values = self.data.view(torch.float8_e4m3fn)
+        return view
 
     def to(self, device) -> "Fp8GroupOperand":
         return Fp8GroupOperand.from_parts(self.data.to(device), self.scales.to(device))
