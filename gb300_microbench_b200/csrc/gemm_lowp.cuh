@@ -190,7 +190,6 @@ struct Params {
   int64_t sfa_ld;             // FP8 by group: rows of one K block's scales
   int64_t ldd;                // row stride of D in elements
   int32_t d_dtype;            // BB_DTYPE_* of a D written directly
-  int32_t d_vec;              // direct: 16-byte stores keep to alignment
 };
 
 // Instruction descriptors.
@@ -337,43 +336,36 @@ __device__ __forceinline__ void promote32(float* acc, const uint32_t (&v)[32], f
   }
 }
 
-// 32 columns of one row of D from registers, v * s, columns from `n` on left out.
-__device__ __forceinline__ void store_direct32(const Params& p, int row, int col, const float* v, float s) {
-  if (row >= p.m || col >= p.n) return;
-  const int64_t at = row * p.ldd + col;
-  const bool whole = p.d_vec && col + 32 <= p.n;
-  if (p.d_dtype == BB_DTYPE_F32) {
-    float* out = reinterpret_cast<float*>(p.d) + at;
-    if (whole) {
+// 32 rows x 32 columns of D from the registers of a warp (lane = row), v * s:
+// through the warp's 4 KiB of shared memory, so that a store instruction writes
+// 32 columns of one row, whatever D's type, stride and alignment. Rows and
+// columns outside D are left out.
+__device__ __forceinline__ void store_direct32(const Params& p, uint32_t box, int row0, int col, const float* v, float s,
+                                               int lane) {
+  if (row0 >= p.m || col >= p.n) return;  // the whole warp
+  __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        reinterpret_cast<float4*>(out)[j] = make_float4(v[4 * j] * s, v[4 * j + 1] * s, v[4 * j + 2] * s, v[4 * j + 3] * s);
+  for (int j = 0; j < 8; ++j)
+    st_shared_v4(box + lane * 128 + ((j ^ (lane & 7)) << 4), __float_as_uint(v[4 * j] * s), __float_as_uint(v[4 * j + 1] * s),
+                 __float_as_uint(v[4 * j + 2] * s), __float_as_uint(v[4 * j + 3] * s));
+  __syncwarp();
+  const int rows = min(32, p.m - row0);
+  const int64_t at = row0 * p.ldd + col + lane;
+  if (col + lane < p.n) {
+    auto element = [&](int r) { return ld_shared_f32(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4); };
+    if (p.d_dtype == BB_DTYPE_F32) {
+      float* d = reinterpret_cast<float*>(p.d) + at;
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r, d += p.ldd) *d = element(r);
+    } else if (p.d_dtype == BB_DTYPE_F16) {
+      __half* d = reinterpret_cast<__half*>(p.d) + at;
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r, d += p.ldd) *d = __float2half_rn(element(r));
     } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col + j < p.n) out[j] = v[j] * s;
+      __nv_bfloat16* d = p.d + at;
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r, d += p.ldd) *d = __float2bfloat16_rn(element(r));
     }
-    return;
-  }
-  uint32_t pk[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    if (p.d_dtype == BB_DTYPE_F16) {
-      const __half2 h = __floats2half2_rn(v[2 * j] * s, v[2 * j + 1] * s);
-      pk[j] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      pk[j] = pack_bf16x2(v[2 * j] * s, v[2 * j + 1] * s);
-    }
-  }
-  uint16_t* out = reinterpret_cast<uint16_t*>(p.d) + at;
-  if (whole) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      reinterpret_cast<uint4*>(out)[j] = make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col + j < p.n) out[j] = static_cast<uint16_t>(pk[j / 2] >> (16 * (j % 2)));
   }
 }
 
@@ -711,8 +703,8 @@ __global__ void __launch_bounds__(Cfg<kKind, kCG>::THREADS, 1)
           tmem_ld_wait();
           if (report) arrive_leader(&ovl_free[b]);
           if constexpr (kDirect) {
-            store_direct32(p, row, col0 + 32 * c, reinterpret_cast<const float*>(r0), scale);
-            store_direct32(p, row, col0 + 32 * (c + 1), reinterpret_cast<const float*>(r1), scale);
+            store_direct32(p, ebuf, row - lane, col0 + 32 * c, reinterpret_cast<const float*>(r0), scale, lane);
+            store_direct32(p, ebuf, row - lane, col0 + 32 * (c + 1), reinterpret_cast<const float*>(r1), scale, lane);
           } else {
             pack32(reinterpret_cast<const float*>(r0), scale, pk + 16 * c);
             pack32(reinterpret_cast<const float*>(r1), scale, pk + 16 * (c + 1));
@@ -735,8 +727,12 @@ __global__ void __launch_bounds__(Cfg<kKind, kCG>::THREADS, 1)
         const int mb = min(m_blk * kCG + static_cast<int>(rank), p.rb_m - 1);
         const int nb = min(col0 / 128, p.rb_n - 1);
         const float* sa_row = sa + static_cast<int64_t>(mb) * p.k_stages;
-        // By group: lane = row, so the lane's own scale of every K block; four
-        // loads ahead, as far as an L2 round trip is in 512-clock blocks with room.
+        // By group: lane = row, so the lane's own scale of every K block, four
+        // loads ahead in a queue. The epilogue's time per block is what the
+        // kernel is made of (8192^3: 538 us back to back, 480 alone, where the
+        // block-scaled form takes 450 and 455), and everything that adds
+        // instructions to it was slower: sets of four scales with selects 620,
+        // a ring in shared memory 610, the loop unrolled by four 620.
         constexpr bool kGroup = kKind == kFp8Group;
         constexpr int kAhead = 4;
         const float* sa_lane = sa + min(row, p.m - 1);
@@ -816,7 +812,7 @@ __global__ void __launch_bounds__(Cfg<kKind, kCG>::THREADS, 1)
 #pragma unroll
         for (int c = 0; c < C::WARP_COLS / 32; ++c) {
           if constexpr (kDirect) {
-            store_direct32(p, row, col0 + 32 * c, acc + 32 * c, scale);
+            store_direct32(p, ebuf, row - lane, col0 + 32 * c, acc + 32 * c, scale, lane);
           } else {
             pack32(acc + 32 * c, scale, pk + 16 * c);
           }

@@ -867,7 +867,6 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
       p.d = static_cast<__nv_bfloat16*>(d);
       p.d_dtype = d_dtype;
       const bool rows16 = reinterpret_cast<uintptr_t>(d) % 16 == 0 && (ldd * d_size) % 16 == 0;
-      p.d_vec = rows16;
       // TMA stores want 16-byte rows; other types and strides are written from registers.
       h->direct = d_dtype != BB_DTYPE_BF16 || !rows16;
       h->grid = p.num_clusters * h->cg;
