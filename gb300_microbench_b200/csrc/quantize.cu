@@ -330,8 +330,8 @@ struct Fp4Params {
   uint8_t* data;           // rows x cols / 2
   uint8_t* atoms;
   void* values;            // dequantised values, may be null
-  const float* partial_max;  // NVFP4 with a scale to be found: the row ranges' maxima
-  int32_t partials;
+  uint32_t* maxima;        // NVFP4 with a scale to be found: the CTAs' maxima, or null
+  unsigned* finished;      // CTAs that wrote theirs, 0 between launches
   float tensor_scale;      // NVFP4 with a given scale
   float* tensor_scale_out;
 };
@@ -418,25 +418,14 @@ __device__ __forceinline__ void put(T* p, const Vec<T>& v) {
   }
 }
 
-__device__ __forceinline__ float found_scale(const float* partial, int n) {
-  // Whole block: the maximum of the partial maxima (bit patterns of
-  // non-negative floats order like the floats, a NaN above all).
-  __shared__ uint32_t warp_max[kFp4Threads / 32];
-  uint32_t m = 0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) m = max(m, __float_as_uint(partial[i]));
-  m = __reduce_max_sync(0xffffffffu, m);
-  if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = m;
-  __syncthreads();
-  for (int i = 0; i < kFp4Threads / 32; ++i) m = max(m, warp_max[i]);
-  const float amax = __uint_as_float(m);
-  const float g = __fdiv_rn(amax, kE4m3Max * kE2m1Max);
-  return g > 0.f ? g : 1.f;  // no data, data below 2688 times the least FP32 number, or NaN
-}
-
-// Maxima of |x| over ranges of the tensor, one per CTA.
+// The tensor scale of NVFP4: maxima of |x| over ranges of the tensor, one per
+// CTA; the CTA that finishes last takes the maximum of all and writes the
+// scale, so the quantising launch reads one word. (Bit patterns of
+// non-negative floats order like the floats, a NaN above all.)
 template <typename T, bool kWide>
-__global__ void __launch_bounds__(kFp4Threads) absmax_kernel(const Fp4Params p, float* partial) {
+__global__ void __launch_bounds__(kFp4Threads) absmax_kernel(const Fp4Params p) {
   __shared__ uint32_t warp_max[kFp4Threads / 32];
+  __shared__ bool last;
   grid_wait();
   grid_trigger();
   const int vecs = p.cols / kVE<T>;  // cols % 32 == 0
@@ -447,12 +436,28 @@ __global__ void __launch_bounds__(kFp4Threads) absmax_kernel(const Fp4Params p, 
     for (int v = threadIdx.x; v < vecs; v += blockDim.x)
       m = max(m, __float_as_uint(absmax(get<kWide>(x + v * kVE<T>))) & 0x7fffffffu);
   }
-  m = __reduce_max_sync(0xffffffffu, m);
-  if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = m;
-  __syncthreads();
+  auto block_max = [&](uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = v;
+    __syncthreads();
+    for (int i = 0; i < kFp4Threads / 32; ++i) v = max(v, warp_max[i]);
+    return v;
+  };
+  m = block_max(m);
   if (threadIdx.x == 0) {
-    for (int i = 1; i < kFp4Threads / 32; ++i) m = max(m, warp_max[i]);
-    partial[blockIdx.x] = __uint_as_float(m);
+    p.maxima[blockIdx.x] = m;
+    __threadfence();
+    last = atomicInc(p.finished, gridDim.x - 1) == gridDim.x - 1;  // back to 0 for the next launch
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  m = 0;
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += blockDim.x) m = max(m, __ldcg(p.maxima + i));
+  m = block_max(m);
+  if (threadIdx.x == 0) {
+    const float g = __fdiv_rn(__uint_as_float(m), kE4m3Max * kE2m1Max);
+    *p.tensor_scale_out = g > 0.f ? g : 1.f;  // no data, data below 2688 times the least FP32 number, or NaN
   }
 }
 
@@ -465,16 +470,13 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quant_kernel(const Fp4Params 
   grid_trigger();
   float g = p.tensor_scale;
   if constexpr (!kMx) {
-    if (p.partial_max) {
-      g = found_scale(p.partial_max, p.partials);
-      if (blockIdx.x == 0 && threadIdx.x == 0) *p.tensor_scale_out = g;
-    }
+    if (p.maxima) g = *p.tensor_scale_out;
   }
   constexpr int kLanes = kMx ? 8 : 4;  // threads of one row's part of an atom
   const uint32_t per_row = static_cast<uint32_t>(p.atoms_k) * kLanes;
   // With a scale found by the launch before, the tensor is read a second time:
   // from its end, which is what L2 still holds of the first reading.
-  const uint32_t block = p.partial_max ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const uint32_t block = p.maxima ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
   const uint32_t idx = block * kFp4Threads + threadIdx.x;
   const bool live = idx < p.total;
   const uint32_t row32 = live ? idx / per_row : 0;
@@ -571,8 +573,7 @@ struct bb_quant_plan {
   NormParams np{};
   Fp4Params fp{};
   int threads = 0, iters = 0;  // RMS norm: vectors per thread, 0 for the widest rows
-  float* partial = nullptr;  // maxima of the NVFP4 tensor scale
-  int partials = 0;
+  int partials = 0;  // CTAs of the launch that finds the NVFP4 tensor scale
   int64_t launches = 0;
 };
 
@@ -614,7 +615,7 @@ template <typename T, bool kWide>
 cudaError_t launch_fp4(const bb_quant_plan& pl) {
   const bool mx = pl.fmt == BB_LOWP_MXFP4;
   if (pl.partials) {
-    const cudaError_t e = launch(absmax_kernel<T, kWide>, pl.partials, kFp4Threads, pl.stream, pl.fp, pl.partial);
+    const cudaError_t e = launch(absmax_kernel<T, kWide>, pl.partials, kFp4Threads, pl.stream, pl.fp);
     if (e != cudaSuccess) return e;
   }
   const unsigned grid = (pl.fp.total + kFp4Threads - 1) / kFp4Threads;
@@ -711,13 +712,15 @@ BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, cons
     if (find && rows > 0) {
       const int64_t most = 8ll * dev.sm_count < kMaxPartials ? 8ll * dev.sm_count : kMaxPartials;
       h->partials = static_cast<int>(rows < most ? rows : most);
-      rc = check_cuda(cudaMalloc(&h->partial, h->partials * sizeof(float)), "cudaMalloc(maxima)");
+      const size_t bytes = (h->partials + 1) * sizeof(uint32_t);
+      rc = check_cuda(cudaMalloc(&p.maxima, bytes), "cudaMalloc(maxima)");
+      if (rc == BB_OK) rc = check_cuda(cudaMemset(p.maxima, 0, bytes), "cudaMemset(maxima)");
       if (rc != BB_OK) {
+        if (p.maxima) cudaFree(p.maxima);
         delete h;
         return rc;
       }
-      p.partial_max = h->partial;
-      p.partials = h->partials;
+      p.finished = p.maxima + h->partials;
     }
     *plan = h;
     return BB_OK;
@@ -859,7 +862,7 @@ BB_API int64_t bb_quant_launches(const bb_quant_plan* plan) { return plan ? plan
 BB_API int bb_quant_destroy(bb_quant_plan* plan) {
   if (!plan) return BB_OK;
   int rc = BB_OK;
-  if (plan->partial) rc = check_cuda(cudaFree(plan->partial), "cudaFree(maxima)");
+  if (plan->fp.maxima) rc = check_cuda(cudaFree(plan->fp.maxima), "cudaFree(maxima)");
   delete plan;
   return rc;
 }

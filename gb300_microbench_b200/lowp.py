@@ -573,6 +573,7 @@ class LowpLinearPlan:
             if not op.data.is_contiguous() or op.data.numel() * op.data.element_size() < op.rows * row_bytes:
                 raise ValueError(f"{name} data must be contiguous and hold {op.rows} x {row_bytes} bytes")
         self._lib = nat.bench_lib()
+        self._execute = self._lib.bb_linear_execute_n
         sx_ld = self.m
         if fp8:
             if tuple(sx.shape) != (self.m, -(-self.k // 128)) or (self.m > 1 and sx.stride(0) != 1) or (
@@ -606,7 +607,9 @@ class LowpLinearPlan:
 
     def run(self, iterations: int = 1) -> None:
         """`iterations` back-to-back launches on the plan's stream (async)."""
-        nat.check("bb_linear_execute_n", self._lib.bb_linear_execute_n(self._handle, int(iterations)))
+        status = self._execute(self._handle, iterations)
+        if status:
+            nat.check("bb_linear_execute_n", status)
 
     def synchronize(self) -> None:
         """Waits for the stream; raises on a device-side wait timeout."""

@@ -50,7 +50,9 @@ class _QuantPlan:
 
     def run(self, iterations: int = 1) -> None:
         """`iterations` back-to-back runs on the plan's stream (async)."""
-        nat.check("bb_quant_execute_n", self._lib.bb_quant_execute_n(self._handle, int(iterations)))
+        status = self._execute(self._handle, iterations)
+        if status:
+            nat.check("bb_quant_execute_n", status)
 
     def synchronize(self) -> None:
         nat.check("bb_quant_synchronize", self._lib.bb_quant_synchronize(self._handle))
@@ -110,6 +112,7 @@ class RmsNormFp8Plan(_QuantPlan):
         self.stream = _one_device(tensors, stream)
         self.x, self.out, self.residual_out, self._keep = x, out, residual_out, tensors
         self._lib = nat.bench_lib()
+        self._execute = self._lib.bb_quant_execute_n
         handle = ctypes.c_void_p()
         with torch.cuda.device(x.device):
             nat.check("bb_rmsnorm_fp8_plan_create", self._lib.bb_rmsnorm_fp8_plan_create(
@@ -157,6 +160,7 @@ class Fp4QuantPlan(_QuantPlan):
         self.stream = _one_device(tensors, stream)
         self.x, self.out, self.values, self._keep = x, out, values, tensors
         self._lib = nat.bench_lib()
+        self._execute = self._lib.bb_quant_execute_n
         handle = ctypes.c_void_p()
         with torch.cuda.device(x.device):
             nat.check("bb_fp4_quant_plan_create", self._lib.bb_fp4_quant_plan_create(
