@@ -145,6 +145,104 @@ def test_strided_output(cuda_device, kind, dtype, m, n, pad, shift):
     assert torch.equal(full.cpu(), want)
 
 
+# More than one tile of 128 x 128 per SM: the kernel of 256 x 256 tiles.
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n,k", [(1921, 1300, 288), (257, 12808, 144), (2048, 2048, 1040), (16100, 200, 96),
+                                   (1400, 1801, 32)])
+def test_exact_many_tiles(cuda_device, kind, m, n, k):
+    gen = torch.Generator().manual_seed(m)
+    k = _round_up(k, kind)
+    x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+    want = _decode(x) @ _decode(w).T
+    d = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device=cuda_device)
+    plan = lowp.LowpLinearPlan(x.to(cuda_device), w.to(cuda_device), d)
+    assert plan.info["few_rows"] == 0
+    plan.run()
+    plan.synchronize()
+    assert torch.equal(d.cpu(), want.float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", list(HALF_STEP))
+@pytest.mark.parametrize("pad,shift", [(0, 0), (3, 1), (8, 8)])
+def test_many_tiles_strided_output(cuda_device, kind, dtype, pad, shift):
+    gen = torch.Generator().manual_seed(pad)
+    m, n, k = 1500, 1700, 160
+    x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+    full = torch.full((m + 2, n + pad + shift), -7.0, dtype=dtype, device=cuda_device)
+    d = full[1:1 + m, shift:shift + n]
+    plan = lowp.LowpLinearPlan(x.to(cuda_device), w.to(cuda_device), d)
+    assert plan.info["few_rows"] == 0
+    plan.run()
+    plan.synchronize()
+    want = torch.full(full.shape, -7.0, dtype=dtype)
+    want[1:1 + m, shift:shift + n] = (_decode(x) @ _decode(w).T).float().to(dtype)
+    assert torch.equal(full.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", list(HALF_STEP))
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_tiles_quantised(cuda_device, kind, dtype):
+    gen = torch.Generator().manual_seed(77)
+    x, w = _quantised_operand(kind, 2100, 2080, gen, False), _quantised_operand(kind, 1430, 2080, gen, True)
+    _check(x, w, _run(x, w, cuda_device, dtype))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_weights_written_just_before(cuda_device, kind):
+    """Launches overlap the ones before them: weights and tokens filled by the launch right in front must
+    be the ones multiplied, every time."""
+    gen = torch.Generator().manual_seed(3)
+    for m, n, k in ((1, 2048, 1024), (40, 1000, 512), (2000, 1664, 256)):
+        x = _quantised_operand(kind, m, k, gen, False).to(cuda_device)
+        sets = [_quantised_operand(kind, n, k, gen, True).to(cuda_device) for _ in range(4)]
+        w = _quantised_operand(kind, n, k, gen, True).to(cuda_device)
+        scales = (lambda op: op.scales) if kind == "fp8" else (lambda op: op.atoms)
+        if kind == "nvfp4":
+            for op in sets:
+                op.tensor_scale = w.tensor_scale
+        outs = [torch.empty(m, n, dtype=torch.bfloat16, device=cuda_device) for _ in sets]
+        plans = [lowp.LowpLinearPlan(x, w, d) for d in outs]
+        own = [lowp.LowpLinearPlan(x, op, torch.empty_like(outs[0])) for op in sets]
+        for _ in range(3):
+            for op, plan in zip(sets, plans):
+                w.data.copy_(op.data)
+                scales(w).copy_(scales(op))
+                plan.run()
+        for p in own:
+            p.run()
+        torch.cuda.synchronize(cuda_device)
+        for d, p in zip(outs, own):
+            assert torch.equal(d, p.d)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_weights_quantised_just_before(cuda_device, fmt):
+    """A weight update: new weights quantised by the plan in front of the product, which starts early."""
+    gen = torch.Generator().manual_seed(4)
+    make = lowp.Mxfp4Operand if fmt == "mxfp4" else lowp.Nvfp4Operand
+    n, k = 1536, 2048
+    src = torch.empty(n, k, dtype=torch.bfloat16, device=cuda_device)
+    w = make.empty(n, k, device=cuda_device)
+    x = _quantised_operand(fmt, 3, k, gen, False).to(cuda_device)
+    d = torch.empty(3, n, dtype=torch.float32, device=cuda_device)
+    fill, product = quantize.Fp4QuantPlan(src, w), lowp.LowpLinearPlan(x, w, d)
+    new = [torch.randn(n, k, generator=gen).to(torch.bfloat16).to(cuda_device) * (1 + i) for i in range(5)]
+    got = []
+    for t in new:
+        src.copy_(t)
+        for _ in range(2):
+            fill.run()
+            product.run()
+        got.append(d.clone())
+    torch.cuda.synchronize(cuda_device)
+    for t, g in zip(new, got):
+        ref = make(t.cpu())
+        want = _decode(x.to("cpu")) @ _decode(ref).T
+        bound = 2.0 ** -24 * want.abs() + (k / 32 + 32) * 2.0 ** -22 * (_decode(x.to("cpu")).abs() @ _decode(ref).abs().T)
+        assert ((g.cpu().double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_nan_stays_in_its_row(cuda_device, kind):
     gen = torch.Generator().manual_seed(5)
