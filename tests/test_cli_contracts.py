@@ -57,6 +57,15 @@ def test_umma_cli_usage_errors_exit_2(argv, code):
     assert um.main(argv) == code
 
 
+@pytest.mark.parametrize("argv,code", [(["--help"], 0), (["--formats", "int8"], 2), (["--tokens", "0"], 2),
+                                       (["--tokens", "x"], 2), (["--k", "48"], 2), (["--iterations", "0"], 2),
+                                       (["--nope"], 2)])
+def test_linear_cli_usage(argv, code):
+    from gb300_microbench_b200.cli import linear
+
+    assert linear.main(argv) == code
+
+
 def test_gemm_self_test_and_usage():
     assert gc.main(["--self-test"]) == 0
     assert gc.main(["--iterations", "0"]) == 2
