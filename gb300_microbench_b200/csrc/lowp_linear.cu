@@ -20,13 +20,14 @@ constexpr int kMaxSplits = 8;  // the portable cluster size
 // useful), the TN tokens its N (16 upwards), so one token costs the same weight
 // stream as sixteen and no arithmetic unit decodes a weight. A CTA streams
 // 128 weight rows over one share of K. The `splits` CTAs of a cluster share K;
-// each owns some of the weight rows and adds all CTAs' FP32 partial sums of
-// them, taken over distributed shared memory, in rank order: the result does
-// not depend on timing. Up to 32 tokens the sums are sent (asynchronous stores
-// that signal the owner's barrier: one way across the cluster, 2.4 us for the
-// smallest launch against 3.2 with reading); more tokens are left in shared
-// memory and read (each asynchronous store of 4 bytes updates the barrier:
-// MXFP4 200 x 5000 x 2880 in 3 splits 15.5 us sent, 9.6 us read).
+// each owns some of the weight rows, is sent the other CTAs' FP32 partial sums
+// of them over distributed shared memory (asynchronous stores of four tokens
+// that signal its barrier), and adds them in rank order: the result does not
+// depend on timing. Tiles of 128 tokens leave the sums in shared memory and
+// read them instead, each CTA some of the tokens (MXFP4 128 x 4096 x 4096 in 4
+// splits 8.4 us read, 9.9 sent; up to 64 tokens sending is faster: NVFP4
+// 64 x 8192 x 8192 12.6 against 12.8, FP8 18.0 against 20.0, and one token 2.4
+// against 3.2 for the smallest launch).
 //
 // FP8: the K blocks' FP32 scales are applied as in the tile kernel, each
 // block accumulated alone in one of BUFS TMEM buffers and promoted by the
@@ -51,29 +52,34 @@ struct FewCfg {
   static constexpr int X_BYTES = TN * ROW_BYTES;
   static constexpr int SF_BYTES = ATOMS * SF_ATOM;  // of the weights, and as much of the tokens
   static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + 2 * SF_BYTES;
-  // Partial sums. Sent: [split][token][owned row] (splits * owned rows are 128
-  // and a few) in a place of their own. Read: [token][128 rows] over the ring.
-  static constexpr bool SEND = TN <= 32;
-  static constexpr int SEND_BYTES = SEND ? TN * (128 + kMaxSplits) * 4 : 0;
+  // Partial sums. Sent: the CTA's own and the others', [split][owned row][token]
+  // (splits * owned rows are 128 and a few; the pitch keeps 16-byte accesses of
+  // neighbouring rows on different banks), in a place of their own where that
+  // is small, otherwise over the ring, once every CTA's is idle. Read:
+  // [token][128 rows] over the ring.
+  static constexpr bool SEND = TN <= 64;
+  static constexpr bool OWN_PLACE = TN <= 32;
+  static constexpr int PITCH = TN + 4;
+  static constexpr int SUM_BYTES = SEND ? (128 + kMaxSplits) * PITCH * 4 : TN * 512;
   // FP8: every epilogue warp keeps the scales of SCALE_SLOTS K blocks (its
   // tokens' and, behind them, the weights').
   static constexpr int SCALE_SLOTS = 4;
   static constexpr int SCALE_PITCH = COLS + 4;
   static constexpr int SCALE_BYTES = FP4 ? 0 : EPI_W * SCALE_SLOTS * SCALE_PITCH * 4;
-  static constexpr int TAIL_BYTES = SEND_BYTES + SCALE_BYTES + BAR_BYTES;
+  static constexpr int TAIL_BYTES = (OWN_PLACE ? SUM_BYTES : 0) + SCALE_BYTES + BAR_BYTES;
   static constexpr int LIMIT = CTAS_PER_SM == 2 ? 115712 : SMEM_LIMIT;
   static constexpr int STAGES_FIT = (LIMIT - 1024 - TAIL_BYTES) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_FIT < 8 ? STAGES_FIT : 8;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TAIL_BYTES;
   // FP8: partial buffers. FP4: one accumulator, then the scale columns.
-  static constexpr int BUFS = FP4 ? 1 : TN == 16 ? 4 : TN == 32 ? 3 : 2;
+  static constexpr int BUFS = FP4 ? 1 : TN == 16 ? 4 : TN <= 64 ? 3 : 2;
   static constexpr int SF_COL = TN;
   static constexpr int SF_COLS = ATOMS * 8;
   static constexpr int COLS_USED = FP4 ? TN + SF_COLS : BUFS * TN;
   static constexpr int TMEM = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : 256;
   static_assert(COLS_USED <= 256 && TMEM * CTAS_PER_SM <= 512, "TMEM of the CTAs that share an SM");
   static_assert(STAGES >= 3 && SMEM_BYTES <= LIMIT, "shared memory");
-  static_assert(SEND || TN * 512 <= STAGES * STAGE_BYTES, "partial sums fit the ring");
+  static_assert(OWN_PLACE || SUM_BYTES <= STAGES * STAGE_BYTES, "partial sums fit the ring");
   static_assert((2 * STAGES + BUFS + 3) * 8 <= BAR_BYTES, "barrier area");
   static_assert(BUFS < STAGES, "a stage's barrier tells the epilogue of its block");
 };
@@ -146,10 +152,11 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool v
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
 
-// 4 bytes into a CTA of the cluster (shared::cluster addresses), counted by a
+// 16 bytes into a CTA of the cluster (shared::cluster addresses), counted by a
 // barrier of that CTA.
-__device__ __forceinline__ void st_async_f32(uint32_t addr, float v, uint32_t mbar) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)),
+__device__ __forceinline__ void st_async_v4f(uint32_t addr, const float* v, uint32_t mbar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr),
+               "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
                "r"(mbar)
                : "memory");
 }
@@ -177,8 +184,8 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
   uint8_t* smem_sfw = smem_x + STAGES * C::X_BYTES;
   uint8_t* smem_sfx = smem_sfw + STAGES * C::SF_BYTES;
   uint8_t* tail = smem + STAGES * C::STAGE_BYTES;
-  float* sums = reinterpret_cast<float*>(C::SEND ? tail : smem);
-  if constexpr (C::SEND) tail += C::SEND_BYTES;
+  float* sums = reinterpret_cast<float*>(C::OWN_PLACE ? tail : smem);
+  if constexpr (C::OWN_PLACE) tail += C::SUM_BYTES;
   float* smem_scale = reinterpret_cast<float*>(tail);
   uint64_t* bars = reinterpret_cast<uint64_t*>(tail + C::SCALE_BYTES);
   uint64_t* full = bars;
@@ -195,6 +202,7 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
   const int ks0 = static_cast<int>(static_cast<int64_t>(p.k_stages) * rank / p.splits);
   const int ks1 = static_cast<int>(static_cast<int64_t>(p.k_stages) * (rank + 1) / p.splits);
   const int mine = min(p.owned, 128 - rank * p.owned);  // weight rows this CTA owns
+  const int quads = (min(C::TN, p.m - m0) + 3) / 4;     // the tile's tokens by fours (those behind M are zeros)
 
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tm_w);
@@ -211,7 +219,7 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
     mbar_init(smem_u32(done), 1);
     mbar_init(smem_u32(received), 1);
     fence_mbarrier_init_cluster();
-    if (C::SEND && p.splits > 1) mbar_arrive_expect_tx(smem_u32(received), (p.splits - 1) * mine * p.m * 4);
+    if (C::SEND && p.splits > 1) mbar_arrive_expect_tx(smem_u32(received), (p.splits - 1) * mine * quads * 16);
   }
   if (warp == 1) {
     tmem_alloc<1>(smem_u32(tmem_slot), C::TMEM);
@@ -227,7 +235,7 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
   tc_fence_before();
   __syncthreads();
   // `received` is ready for the other CTAs' signals; waited for before sending.
-  if (C::SEND && p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (C::OWN_PLACE && p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   grid_wait();
@@ -400,19 +408,23 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
         }
       }
       cp_async_wait<0>();
-      if (!C::SEND && p.splits > 1)
+      if (!C::OWN_PLACE && p.splits > 1)
         ok = bb_wait_warp<false, false>(smem_u32(done), 0, p.status, kDevTimeoutEpilogue) && ok;
     }
   }
-  if (C::SEND && p.splits > 1) {
+  if (p.splits > 1) {
     __syncwarp();
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if constexpr (C::OWN_PLACE) {
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else if constexpr (C::SEND) {
+      cluster_sync();  // every CTA's ring is idle (`done`: every copy has landed and been read)
+    }
   }
   if (warp >= 2) {
     // This thread's sums, CHUNK tokens at a time: to D, to the row's owner, or
-    // into the ring, which is idle (`done`: every copy has landed and been read).
+    // into this CTA's ring.
     const int owner = row / p.owned;
-    const uint32_t at = ((rank * C::TN + col0) * p.owned + row - owner * p.owned) * 4;
+    const uint32_t at = ((rank * p.owned + row - owner * p.owned) * C::PITCH + col0) * 4;
     const uint32_t to = mapa_shared(smem_u32(sums) + at, owner), to_bar = mapa_shared(smem_u32(received), owner);
 #pragma unroll
     for (int c0 = 0; c0 < C::COLS; c0 += C::CHUNK) {
@@ -430,16 +442,18 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
       }
       if (p.splits == 1) {
         store_tokens(p, m0 + col0 + c0, min(C::CHUNK, tokens - c0), n, v, scale);
-      } else if constexpr (C::SEND) {
-#pragma unroll
-        for (int c = 0; c < C::CHUNK; ++c) {
-          if (c0 + c >= tokens) continue;
-          if (owner == rank) sums[at / 4 + (c0 + c) * p.owned] = v[c];
-          else st_async_f32(to + (c0 + c) * p.owned * 4, v[c], to_bar);
-        }
-      } else {
+      } else if constexpr (!C::SEND) {
 #pragma unroll
         for (int c = 0; c < C::CHUNK; ++c) sums[(col0 + c0 + c) * 128 + row] = v[c];
+      } else {
+#pragma unroll
+        for (int c = 0; c < C::CHUNK; c += 4) {
+          if (c0 + c >= tokens) continue;
+          if (owner == rank)
+            *reinterpret_cast<float4*>(sums + at / 4 + c0 + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+          else
+            st_async_v4f(to + (c0 + c) * 4, v + c, to_bar);
+        }
       }
       __syncwarp();
     }
@@ -451,26 +465,34 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
     if (warp >= 2) {
       asm volatile("bar.sync 1, %0;" ::"n"(32 * C::EPI_W) : "memory");  // the CTA's own sums
       bb_wait_warp<true, false>(smem_u32(received), 0, p.status, kDevTimeoutEpilogue);
-      // Element e of the m x mine sums, e = thread, thread + threads, ...
+      // Element e of the quads x mine sums of four tokens, e = thread, thread + threads, ...
       constexpr int kThreads = 32 * C::EPI_W;
       const int e0 = threadIdx.x - 64;
-      int token = e0 / mine, r0 = e0 - token * mine;
+      int quad = e0 / mine, r0 = e0 - quad * mine;
       const int step = kThreads / mine, step_row = kThreads - step * mine;
-      while (token < p.m) {
-        const float* from = sums + token * p.owned + r0;
-        float f[kMaxSplits];
+      while (quad < quads) {
+        const float4* from = reinterpret_cast<const float4*>(sums + r0 * C::PITCH) + quad;
+        float4 f[kMaxSplits];
 #pragma unroll
-        for (int r = 0; r < kMaxSplits; ++r) f[r] = r < p.splits ? from[r * C::TN * p.owned] : 0.f;
-        float v = f[0];
+        for (int r = 0; r < kMaxSplits; ++r)
+          if (r < p.splits) f[r] = from[r * p.owned * (C::PITCH / 4)];
+        float v[4] = {f[0].x, f[0].y, f[0].z, f[0].w};
 #pragma unroll
-        for (int r = 1; r < kMaxSplits; ++r) v += f[r];
-        const int at_n = n_blk * 128 + rank * p.owned + r0;
-        if (at_n < p.n) store_one(p.d, p.d_dtype, token * p.ldd + at_n, v * scale);
-        token += step;
+        for (int r = 1; r < kMaxSplits; ++r) {
+          if (r < p.splits) {
+            v[0] += f[r].x;
+            v[1] += f[r].y;
+            v[2] += f[r].z;
+            v[3] += f[r].w;
+          }
+        }
+        const int token = m0 + 4 * quad;
+        store_tokens(p, token, min(4, p.m - token), n_blk * 128 + rank * p.owned + r0, v, scale);
+        quad += step;
         r0 += step_row;
         if (r0 >= mine) {
           r0 -= mine;
-          ++token;
+          ++quad;
         }
       }
     }
