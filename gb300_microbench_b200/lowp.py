@@ -541,7 +541,9 @@ class LowpLinearPlan:
     weights (K a multiple of 16). D is bfloat16, float16 or float32 with
     unit column stride and row stride >= N; its bytes outside (M, N) are not
     touched. Tensor scales found on the GPU (``tensor_scale_out``) are read there
-    at every run. The plan keeps its operands; x may be refilled between runs."""
+    at every run. The plan keeps its operands; x and w may be refilled between
+    runs by work on the plan's stream. Runs can be captured into a CUDA graph,
+    which then needs the plan to stay alive."""
 
     def __init__(self, x, w, d: torch.Tensor, stream: torch.cuda.Stream | None = None):
         if type(x) not in _LINEAR_KINDS:
@@ -607,7 +609,7 @@ class LowpLinearPlan:
 
     def run(self, iterations: int = 1) -> None:
         """`iterations` back-to-back launches on the plan's stream (async)."""
-        status = self._execute(self._handle, iterations)
+        status = self._execute(self._handle, int(iterations))
         if status:
             nat.check("bb_linear_execute_n", status)
 

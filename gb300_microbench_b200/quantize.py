@@ -4,7 +4,8 @@ and the 4-bit microscaled formats. They fill the operands that
 
 Like the GEMM plans, a plan is built once for fixed tensors and run many
 times on its stream; the tensors stay the caller's, and x may hold new data at
-every run. ``lowp.nvfp4_quantize``, ``lowp.mxfp4_quantize`` and
+every run. Runs can be captured into a CUDA graph, which then needs the plan
+(and its tensors) to stay alive; a plan's runs belong to one stream at a time. ``lowp.nvfp4_quantize``, ``lowp.mxfp4_quantize`` and
 ``lowp.fp8_group_quantize`` are the same formats in torch; the 4-bit
 kernels equal them bit for bit (on the CPU, where torch divides exactly).
 """
@@ -50,7 +51,7 @@ class _QuantPlan:
 
     def run(self, iterations: int = 1) -> None:
         """`iterations` back-to-back runs on the plan's stream (async)."""
-        status = self._execute(self._handle, iterations)
+        status = self._execute(self._handle, int(iterations))
         if status:
             nat.check("bb_quant_execute_n", status)
 

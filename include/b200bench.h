@@ -319,7 +319,9 @@ typedef struct bb_linear_plan bb_linear_plan;
 /* Bytes of a scale operand: of the weights (weights != 0, rows = N) or of the
  * activations (rows = M; FP8_GROUP128: with sfa_ld = rows), or -1. */
 BB_API int64_t bb_linear_scale_bytes(int kind, int weights, int64_t rows, int64_t k);
-/* info->reserved[0]: 1 when the kernel for few rows runs; [1]: its K splits. */
+/* info->reserved[0]: 1 when the kernel for few rows runs; [1]: its K splits.
+ * A plan's launches (and the CUDA graphs that captured them, which need the
+ * plan alive) belong to one stream at a time. */
 BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, const void* a, const void* b,
                                  const void* sfa, int64_t sfa_ld, const void* sfb, float scale_a,
                                  const float* scale_a_dev, float scale_b, const float* scale_b_dev, void* d,

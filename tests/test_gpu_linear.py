@@ -351,3 +351,41 @@ def test_refusals_on_the_gpu(cuda_device):
         plan.run(-1)
     plan.run(0)
     assert plan.launches == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_output_stride_past_32_bits(cuda_device, kind):
+    """Rows of D 2^31 elements apart."""
+    gen = torch.Generator().manual_seed(6)
+    m, n, k = 3, 200, 96
+    x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+    big = torch.empty(2 * (1 << 31) + n, dtype=torch.bfloat16, device=cuda_device)
+    d = big.as_strided((m, n), (1 << 31, 1))
+    plan = lowp.LowpLinearPlan(x.to(cuda_device), w.to(cuda_device), d)
+    plan.run()
+    plan.synchronize()
+    assert torch.equal(d.cpu(), (_decode(x) @ _decode(w).T).float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_large_output(cuda_device, kind):
+    """More than 2^32 elements of D (the tile kernel): identical rows of x give identical rows of D."""
+    gen = torch.Generator().manual_seed(7)
+    m, n, k = 66000, 65600, 64
+    base = _exact_operand(kind, 200, k, gen, False)
+    w = _exact_operand(kind, n, k, gen, True).to(cuda_device)
+    reps = m // 200
+    if kind == "fp8":
+        x = lowp.Fp8GroupOperand.from_parts(base.data.repeat(reps, 1), base.scales.repeat(reps, 1))
+    else:
+        bits = lowp.unpack_scale_atoms(base.atoms, 200, k // (32 if kind == "mxfp4" else 16))
+        parts = (base.data.repeat(reps, 1), bits.repeat(reps, 1))
+        x = lowp.Mxfp4Operand.from_parts(*parts) if kind == "mxfp4" else lowp.Nvfp4Operand.from_parts(*parts, base.tensor_scale)
+    d = torch.empty(m, n, dtype=torch.bfloat16, device=cuda_device)
+    plan = lowp.LowpLinearPlan(x.to(cuda_device), w, d)
+    assert plan.info["few_rows"] == 0
+    plan.run()
+    plan.synchronize()
+    first = (_decode(base) @ _decode(w.to("cpu")).T).float().to(torch.bfloat16).to(cuda_device)
+    for rep in (0, reps // 2, reps - 1):
+        assert torch.equal(d[200 * rep:200 * rep + 200], first)

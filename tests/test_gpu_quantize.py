@@ -284,3 +284,76 @@ def test_other_stream_and_graph(cuda_device):
         packed, bits, g, _ = _fp4_reference("nvfp4", new)
         assert torch.equal(nv.data.cpu(), packed) and torch.equal(nv.atoms.cpu(), lowp.pack_scale_atoms(bits))
         assert float(nv.tensor_scale_out) == float(torch.tensor(g, dtype=torch.float32))
+
+
+def test_row_strides_past_32_bits(cuda_device):
+    """Rows 2^31 elements apart."""
+    ld, cols = 1 << 31, 288
+    big = torch.empty(ld + cols, dtype=torch.bfloat16, device=cuda_device)
+    x = big.as_strided((2, cols), (ld, 1))
+    src = _x(2, cols, torch.bfloat16, seed=40)
+    x.copy_(src.to(cuda_device))
+    w = torch.ones(cols)
+    out = lowp.Fp8GroupOperand.empty(2, cols, device=cuda_device)
+    plan = quantize.RmsNormFp8Plan(x, w.to(cuda_device), out, residual=x, residual_out=x)  # h = 2 x, in place
+    plan.run()
+    plan.synchronize()
+    _norm_check(src, src, w, 1e-6, x.cpu(), out.values.float().cpu(), out.scales.cpu())
+    for fmt in ("mxfp4", "nvfp4"):
+        x.copy_(src.to(cuda_device))
+        packed, bits, _, deq = _fp4_reference(fmt, src)
+        op = _operand(fmt, 2, cols, cuda_device, None)
+        plan = quantize.Fp4QuantPlan(x, op, values=x)
+        plan.run()
+        plan.synchronize()
+        assert torch.equal(op.data.cpu(), packed) and torch.equal(x.cpu(), deq.to(torch.bfloat16))
+
+
+def test_tensors_past_32_bits(cuda_device):
+    """More than 2^32 elements of x: the last rows against the first."""
+    rows, cols = 524289, 8192
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=cuda_device)
+    x.view(-1)[: 128 * cols].copy_(_x(128, cols, torch.bfloat16, seed=41).to(cuda_device).view(-1))
+    x[128:] = 0
+    x[-1].copy_(x[77])
+    x[rows // 2 + 1].copy_(x[3])
+    op = lowp.Mxfp4Operand.empty(rows, cols, device=cuda_device)
+    plan = quantize.Fp4QuantPlan(x, op)
+    plan.run()
+    plan.synchronize()
+    bits = lowp.unpack_scale_atoms(op.atoms[-1:], 1, cols // 32)
+    first = lowp.unpack_scale_atoms(op.atoms[:1], 128, cols // 32)
+    assert torch.equal(op.data[-1], op.data[77]) and torch.equal(bits[0], first[77])
+    assert torch.equal(op.data[rows // 2 + 1], op.data[3]) and not op.data[rows // 2 + 2].any()
+    out = lowp.Fp8GroupOperand.empty(rows, cols, device=cuda_device)
+    plan = quantize.RmsNormFp8Plan(x, torch.ones(cols, device=cuda_device), out)
+    plan.run()
+    plan.synchronize()
+    assert torch.equal(out.data[-1], out.data[77]) and torch.equal(out.scales[-1], out.scales[77])
+    assert torch.equal(out.data[rows // 2 + 1], out.data[3]) and not out.data[rows // 2 + 2].any()
+
+
+def test_graphs_of_one_plan(cuda_device):
+    """Two graphs captured from one plan, replayed in turn; then a closed plan refuses."""
+    stream = torch.cuda.Stream(device=cuda_device)
+    x = torch.empty(200, 512, dtype=torch.float16, device=cuda_device)
+    op = lowp.Nvfp4Operand.empty(200, 512, device=cuda_device)
+    plan = quantize.Fp4QuantPlan(x, op, stream=stream)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for n, graph in enumerate(graphs):
+        with torch.cuda.graph(graph, stream=stream):
+            plan.run(n + 1)
+    for i, scale in enumerate((1.0, 5.0, 0.01, 300.0)):
+        new = _x(200, 512, torch.float16, seed=50 + i) * scale
+        x.copy_(new.to(cuda_device))
+        torch.cuda.synchronize(cuda_device)
+        with torch.cuda.stream(stream):
+            graphs[i % 2].replay()
+        stream.synchronize()
+        packed, bits, g, _ = _fp4_reference("nvfp4", new)
+        assert torch.equal(op.data.cpu(), packed) and torch.equal(op.atoms.cpu(), lowp.pack_scale_atoms(bits))
+    del graphs
+    plan.close()
+    from gb300_microbench_b200 import _native as nat
+    with pytest.raises(nat.NativeCallError):
+        plan.run()
