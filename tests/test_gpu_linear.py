@@ -389,3 +389,49 @@ def test_large_output(cuda_device, kind):
     first = (_decode(base) @ _decode(w.to("cpu")).T).float().to(torch.bfloat16).to(cuda_device)
     for rep in (0, reps // 2, reps - 1):
         assert torch.equal(d[200 * rep:200 * rep + 200], first)
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "fp8"])
+def test_captured_fork_and_join(cuda_device, kind):
+    """The layer inside a graph whose streams fork and join around it: copies and kernels of other streams
+    in front of it, readers behind it."""
+    gen = torch.Generator().manual_seed(8)
+    m, k, n = 20, 512, 640
+    main, side = torch.cuda.Stream(device=cuda_device), torch.cuda.Stream(device=cuda_device)
+    w = _quantised_operand(kind, n, k, gen, True).to(cuda_device)
+    src = torch.empty(m, k, dtype=torch.bfloat16, device=cuda_device)
+    x, res = torch.empty_like(src), torch.empty_like(src)
+    d, behind = (torch.empty(m, n, dtype=torch.bfloat16, device=cuda_device) for _ in range(2))
+    if kind == "fp8":
+        a = lowp.Fp8GroupOperand.empty(m, k, device=cuda_device)
+        first = quantize.RmsNormFp8Plan(x, torch.ones(k, device=cuda_device), a, residual=res, stream=main)
+    else:
+        a = lowp.Mxfp4Operand.empty(m, k, device=cuda_device)
+        first = quantize.Fp4QuantPlan(x, a, stream=main)
+    product = lowp.LowpLinearPlan(a, w, d, stream=main)
+    torch.cuda.synchronize(cuda_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            x.copy_(src)
+            res.copy_(src)
+            res.mul_(0.5)
+        main.wait_stream(side)
+        first.run()
+        product.run()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            behind.copy_(d)
+        product.run()
+        main.wait_stream(side)
+        d.zero_()
+    for i in range(3):
+        src.copy_(torch.randn(m, k, generator=gen).to(torch.bfloat16) * (i + 1))
+        torch.cuda.synchronize(cuda_device)
+        graph.replay()
+        torch.cuda.synchronize(cuda_device)
+        assert not d.any()
+        _check(a.to("cpu"), w.to("cpu"), behind.cpu())
+        if kind == "mxfp4":
+            assert torch.equal(a.data.cpu(), lowp.mxfp4_quantize(src.cpu())[0])
