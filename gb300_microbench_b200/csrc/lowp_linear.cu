@@ -33,6 +33,11 @@ constexpr int kMaxSplits = 8;  // the portable cluster size
 // block accumulated alone in one of BUFS TMEM buffers and promoted by the
 // epilogue warps: acc[c] += part[c] * sb[kb] * sa[token c][kb].
 //
+// FP8 tiles of 128 tokens turn the product round (tokens on M, weights on N):
+// a lane then holds one token, so a K block has one scale per lane instead of
+// one per column, whose 64 shared-memory broadcasts per warp stood in the way of
+// the operand traffic (256 x 8192 x 8192: 37 us before, 29 after).
+//
 // What bounds it is the weight stream, and then the ends of the launch: two
 // CTAs of up to 113 KiB share an SM (TN <= 128), so about 200 KiB of weights
 // per SM are in flight, and CTAs of the next launch start beside the last
@@ -41,6 +46,7 @@ template <int kKind, int kTN>
 struct FewCfg {
   static constexpr int TN = kTN;
   static constexpr bool FP4 = is_fp4(kKind);
+  static constexpr bool TURNED = !FP4 && TN == 128;  // tokens on M
   static constexpr int CTAS_PER_SM = FP4 || TN <= 64 ? 2 : 1;  // FP8's 64 accumulators a thread want a whole SM's registers
   static constexpr int EPI_W = TN <= 32 ? 4 : 8;  // epilogue warps: lane quarters x column halves
   static constexpr int THREADS = 64 + 32 * EPI_W;
@@ -56,15 +62,17 @@ struct FewCfg {
   // (splits * owned rows are 128 and a few; the pitch keeps 16-byte accesses of
   // neighbouring rows on different banks), in a place of their own where that
   // is small, otherwise over the ring, once every CTA's is idle. Read:
-  // [token][128 rows] over the ring.
+  // [token][128 rows] over the ring (turned tiles too, whose lanes are tokens:
+  // four words more a token keep their writes on different banks).
   static constexpr bool SEND = TN <= 64;
   static constexpr bool OWN_PLACE = TN <= 32;
-  static constexpr int PITCH = TN + 4;
-  static constexpr int SUM_BYTES = SEND ? (128 + kMaxSplits) * PITCH * 4 : TN * 512;
+  static constexpr int PITCH = SEND ? TN + 4 : TURNED ? 132 : 128;
+  static constexpr int SUM_BYTES = (SEND ? 128 + kMaxSplits : TN) * PITCH * 4;
   // FP8: every epilogue warp keeps the scales of SCALE_SLOTS K blocks (its
   // tokens' and, behind them, the weights').
   static constexpr int SCALE_SLOTS = 4;
-  static constexpr int SCALE_PITCH = COLS + 4;
+  static constexpr int SCALES = TURNED ? 32 : COLS;  // token scales of a warp and K block
+  static constexpr int SCALE_PITCH = SCALES + 4;
   static constexpr int SCALE_BYTES = FP4 ? 0 : EPI_W * SCALE_SLOTS * SCALE_PITCH * 4;
   static constexpr int TAIL_BYTES = (OWN_PLACE ? SUM_BYTES : 0) + SCALE_BYTES + BAR_BYTES;
   static constexpr int LIMIT = CTAS_PER_SM == 2 ? 115712 : SMEM_LIMIT;
@@ -72,12 +80,12 @@ struct FewCfg {
   static constexpr int STAGES = STAGES_FIT < 8 ? STAGES_FIT : 8;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TAIL_BYTES;
   // FP8: partial buffers. FP4: one accumulator, then the scale columns.
-  static constexpr int BUFS = FP4 ? 1 : TN == 16 ? 4 : TN <= 64 ? 3 : 2;
+  static constexpr int BUFS = FP4 ? 1 : TN == 16 || TN == 128 ? 4 : 3;
   static constexpr int SF_COL = TN;
   static constexpr int SF_COLS = ATOMS * 8;
   static constexpr int COLS_USED = FP4 ? TN + SF_COLS : BUFS * TN;
-  static constexpr int TMEM = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : 256;
-  static_assert(COLS_USED <= 256 && TMEM * CTAS_PER_SM <= 512, "TMEM of the CTAs that share an SM");
+  static constexpr int TMEM = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
+  static_assert(COLS_USED <= TMEM && TMEM * CTAS_PER_SM <= 512, "TMEM of the CTAs that share an SM");
   static_assert(STAGES >= 3 && SMEM_BYTES <= LIMIT, "shared memory");
   static_assert(OWN_PLACE || SUM_BYTES <= STAGES * STAGE_BYTES, "partial sums fit the ring");
   static_assert((2 * STAGES + BUFS + 3) * 8 <= BAR_BYTES, "barrier area");
@@ -106,6 +114,26 @@ __device__ __forceinline__ void store_one(void* d, int dtype, int64_t at, float 
   if (dtype == BB_DTYPE_BF16) static_cast<__nv_bfloat16*>(d)[at] = __float2bfloat16_rn(v);
   else if (dtype == BB_DTYPE_F16) static_cast<__half*>(d)[at] = __float2half_rn(v);
   else static_cast<float*>(d)[at] = v;
+}
+
+// `count` (none if negative) of four neighbouring columns of D, in one access where it is whole and aligned.
+__device__ __forceinline__ void store_four(const FewParams& p, int64_t at, int count, const float (&v)[4]) {
+  const int bytes = p.d_dtype == BB_DTYPE_F32 ? 4 : 2;
+  uint8_t* d = static_cast<uint8_t*>(p.d) + at * bytes;
+  if (count == 4 && reinterpret_cast<uintptr_t>(d) % (4 * bytes) == 0) {
+    if (p.d_dtype == BB_DTYPE_F32) {
+      *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if (p.d_dtype == BB_DTYPE_F16) {
+      const __half2 lo = __floats2half2_rn(v[0], v[1]), hi = __floats2half2_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(d) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    } else {
+      *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < count) store_one(p.d, p.d_dtype, at + i, v[i]);
 }
 
 // `count` of N tokens of one column of D.
@@ -330,7 +358,8 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
         } else {
 #pragma unroll
           for (int g = 0; g < C::MMAS; ++g)
-            mma_f8<1>(d_tmem, w_desc + 2 * g, x_desc + 2 * g, idesc_f8(128, C::TN), g != 0 ? 1u : 0u);
+            mma_f8<1>(d_tmem, (C::TURNED ? x_desc : w_desc) + 2 * g, (C::TURNED ? w_desc : x_desc) + 2 * g,
+                      idesc_f8(128, C::TN), g != 0 ? 1u : 0u);
         }
         umma_commit<1>(smem_u32(&empty[stage]));
       }
@@ -356,13 +385,15 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
       auto fetch_scales = [&](int ks) {
         if (ks < ks1) {
           const uint32_t dst = smem_u32(my_scale + (ks - ks0) % C::SCALE_SLOTS * C::SCALE_PITCH);
-          const float* src = p.sfa + ks * p.sfa_ld + m0 + col0;
+          const int t0 = C::TURNED ? q * 32 : col0;  // first token of the warp
+          const int count = min(C::SCALES, p.m - m0 - t0);
+          const float* src = p.sfa + ks * p.sfa_ld + m0 + t0;
 #pragma unroll
-          for (int j = 0; j < (C::COLS + 31) / 32; ++j) {
+          for (int j = 0; j < (C::SCALES + 31) / 32; ++j) {
             const int c = lane + 32 * j;
-            if (c < C::COLS) cp_async_4(dst + c * 4, c < tokens ? src + c : p.sfa, c < tokens);
+            if (c < C::SCALES) cp_async_4(dst + c * 4, c < count ? src + c : p.sfa, c < count);
           }
-          if (lane == 31) cp_async_4(dst + C::COLS * 4, p.sfb + static_cast<int64_t>(n_blk) * p.k_stages + ks, true);
+          if (lane == 31) cp_async_4(dst + C::SCALES * 4, p.sfb + static_cast<int64_t>(n_blk) * p.k_stages + ks, true);
         }
         cp_async_commit();
       };
@@ -377,7 +408,8 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
         cp_async_wait<C::SCALE_SLOTS - 1>();
         __syncwarp();
         const float* sc = my_scale + it % C::SCALE_SLOTS * C::SCALE_PITCH;
-        const F2 sb = pack2(sc[C::COLS], sc[C::COLS]);
+        const float s_lane = C::TURNED ? sc[lane] * sc[C::SCALES] : sc[C::SCALES];
+        const F2 s2 = pack2(s_lane, s_lane);  // turned: the lane's whole scale; else the weights'
         // The commit that releases the operand stage also says that the K
         // block's partial is complete; the MMA warp runs at most BUFS < STAGES
         // blocks ahead, so the parity cannot be overtaken.
@@ -399,16 +431,23 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
           }
 #pragma unroll
           for (int c = 0; c < C::CHUNK; c += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(sc + c0 + c);
             F2& a0 = acc[(c0 + c) / 2];
             F2& a1 = acc[(c0 + c) / 2 + 1];
-            a0 = fma2(mul2(pack2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sb), pack2(s.x, s.y), a0);
-            a1 = fma2(mul2(pack2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), sb), pack2(s.z, s.w), a1);
+            const F2 r0 = pack2(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+            const F2 r1 = pack2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
+            if constexpr (C::TURNED) {
+              a0 = fma2(r0, s2, a0);
+              a1 = fma2(r1, s2, a1);
+            } else {
+              const float4 s = *reinterpret_cast<const float4*>(sc + c0 + c);
+              a0 = fma2(mul2(r0, s2), pack2(s.x, s.y), a0);
+              a1 = fma2(mul2(r1, s2), pack2(s.z, s.w), a1);
+            }
           }
         }
       }
       cp_async_wait<0>();
-      if (!C::OWN_PLACE && p.splits > 1)
+      if (C::TURNED || (!C::OWN_PLACE && p.splits > 1))
         ok = bb_wait_warp<false, false>(smem_u32(done), 0, p.status, kDevTimeoutEpilogue) && ok;
     }
   }
@@ -428,7 +467,7 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
     const uint32_t to = mapa_shared(smem_u32(sums) + at, owner), to_bar = mapa_shared(smem_u32(received), owner);
 #pragma unroll
     for (int c0 = 0; c0 < C::COLS; c0 += C::CHUNK) {
-      if (c0 >= tokens) break;
+      if (!C::TURNED && c0 >= tokens) break;
       float v[C::CHUNK];
       if constexpr (C::FP4) {
         uint32_t r[C::CHUNK];
@@ -440,11 +479,15 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
 #pragma unroll
         for (int c = 0; c < C::CHUNK; c += 2) unpack2(acc[(c0 + c) / 2], v[c], v[c + 1]);
       }
-      if (p.splits == 1) {
+      if constexpr (C::TURNED) {
+#pragma unroll
+        for (int c = 0; c < C::CHUNK; c += 4)
+          *reinterpret_cast<float4*>(sums + row * C::PITCH + col0 + c0 + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+      } else if (p.splits == 1) {
         store_tokens(p, m0 + col0 + c0, min(C::CHUNK, tokens - c0), n, v, scale);
       } else if constexpr (!C::SEND) {
 #pragma unroll
-        for (int c = 0; c < C::CHUNK; ++c) sums[(col0 + c0 + c) * 128 + row] = v[c];
+        for (int c = 0; c < C::CHUNK; ++c) sums[(col0 + c0 + c) * C::PITCH + row] = v[c];
       } else {
 #pragma unroll
         for (int c = 0; c < C::CHUNK; c += 4) {
@@ -499,10 +542,11 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
     __syncwarp();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   }
-  if (!C::SEND && p.splits > 1) {
+  if (!C::SEND && (C::TURNED || p.splits > 1)) {
     __syncwarp();
-    cluster_sync();
+    if (p.splits > 1) cluster_sync();
     if (warp >= 2) {
+      if (p.splits == 1) asm volatile("bar.sync 1, %0;" ::"n"(32 * C::EPI_W) : "memory");
       // Rank r adds the tokens r, r + splits, ... of all ranks' partial sums: a
       // warp per token, a lane four weight rows. Remote loads take most of a
       // microsecond each, so those of all ranks and of two tokens are in flight together.
@@ -515,10 +559,10 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
 #pragma unroll
         for (int r = 0; r < kMaxSplits; ++r) {
           if (r >= p.splits) break;
-          const uint32_t from = mapa_shared(base + c * 512, r);
+          const uint32_t from = mapa_shared(base + c * C::PITCH * 4, r);
 #pragma unroll
           for (int j = 0; j < kBatch; ++j)
-            if (c + j * p.splits * C::EPI_W < count) v[j][r] = ld_cluster_v4f(from + j * p.splits * C::EPI_W * 512);
+            if (c + j * p.splits * C::EPI_W < count) v[j][r] = ld_cluster_v4f(from + j * p.splits * C::EPI_W * C::PITCH * 4);
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
@@ -533,16 +577,13 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
             sum.z += v[j][r].z;
             sum.w += v[j][r].w;
           }
-          const int64_t at = (m0 + token) * p.ldd + n4;
           const float out[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n4 + i < p.n) store_one(p.d, p.d_dtype, at + i, out[i]);
+          store_four(p, (m0 + token) * p.ldd + n4, min(4, p.n - n4), out);
         }
       }
     }
     __syncwarp();
-    cluster_sync();  // no CTA leaves while another reads its partial sums
+    if (p.splits > 1) cluster_sync();  // no CTA leaves while another reads its partial sums
   }
   tc_fence_before();
   __syncthreads();
