@@ -47,7 +47,7 @@ struct FewCfg {
   static constexpr int TN = kTN;
   static constexpr bool FP4 = is_fp4(kKind);
   static constexpr bool TURNED = !FP4 && TN == 128;  // tokens on M
-  static constexpr int CTAS_PER_SM = FP4 || TN <= 64 ? 2 : 1;  // FP8's 64 accumulators a thread want a whole SM's registers
+  static constexpr int CTAS_PER_SM = FP4 || TN <= 32 ? 2 : 1;  // FP8's 64 accumulators a thread want a whole SM's registers
   static constexpr int EPI_W = TN <= 32 ? 4 : 8;  // epilogue warps: lane quarters x column halves
   static constexpr int THREADS = 64 + 32 * EPI_W;
   static constexpr int COLS = TN * 4 / EPI_W;     // accumulator columns per epilogue thread
@@ -80,7 +80,7 @@ struct FewCfg {
   static constexpr int STAGES = STAGES_FIT < 8 ? STAGES_FIT : 8;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TAIL_BYTES;
   // FP8: partial buffers. FP4: one accumulator, then the scale columns.
-  static constexpr int BUFS = FP4 ? 1 : TN == 16 || TN == 128 ? 4 : 3;
+  static constexpr int BUFS = FP4 ? 1 : TN == 32 ? 3 : 4;
   static constexpr int SF_COL = TN;
   static constexpr int SF_COLS = ATOMS * 8;
   static constexpr int COLS_USED = FP4 ? TN + SF_COLS : BUFS * TN;
@@ -664,7 +664,9 @@ int launch_few_kind(const bb_linear_plan& pl) {
   switch (pl.tn) {
     case 16: return launch_few<kKind, 16>(pl);
     case 32: return launch_few<kKind, 32>(pl);
-    case 64: return launch_few<kKind, 64>(pl);
+    case 64:
+      if constexpr (is_fp4(kKind)) return launch_few<kKind, 64>(pl);
+      [[fallthrough]];
     default: return launch_few<kKind, 128>(pl);
   }
 }
@@ -733,19 +735,20 @@ int launch_linear(const bb_linear_plan& pl) {
 // Which kernel: the one for few rows up to 128 rows, and above as long as its
 // 128 x 128 tiles are not more than the SMs. The tile kernel's 256 x 256 pairs
 // would leave most SMs idle there (FP8, few against tiles: 256 x 4096 x 4096
-// 14.7 us / 19.8, 512 x 1024 x 8192 15.0 / 35.2, 512 x 4096 x 4096 20.5 / 20.5;
-// MXFP4 200 x 5000 x 2880 8.7 / 9.7).
+// 12.1 us / 19.8, 512 x 1024 x 8192 12.3 / 35.2, 512 x 4096 x 4096 17.3 / 20.5;
+// MXFP4 200 x 5000 x 2880 8.7 / 9.7), and is faster beyond (FP8 512 x 6144 x 4096
+// 33.0 / 20.3, MXFP4 11.6 / 11.4).
 bool use_few(int64_t m, int64_t rb_n, int sm_count) { return m <= 128 || rb_n * ((m + 127) / 128) <= sm_count; }
 
 // K splits of the few-rows kernel. One CTA per SM suffices for a short K: more
 // of them only add to the exchange (MXFP4 128 x 4096 x 4096, 32 row blocks:
 // 4 splits 8.4 us, 8 splits 12.8). A second CTA per SM keeps more of a long
-// weight stream in flight (NVFP4 1 x 8192 x 8192: 2 splits 10.8 us, 4 splits
-// 9.2; FP8 1 x 14336 x 4096: 1 split 14.6, 2 splits 13.0) where each still has
+// weight stream in flight (NVFP4 1 x 8192 x 8192: 2 splits 10.4 us, 4 splits
+// 8.6; FP8 1 x 14336 x 4096: 1 split 14.4, 2 splits 12.9) where each still has
 // kLongShare stages. Never more CTAs than are resident at once: a second wave
-// costs half the kernel (5 splits of the same NVFP4 case 12.4 us). Sums of
+// costs half the kernel (6 splits of the same NVFP4 case 12.0 us). Sums of
 // many tokens are read from at most six CTAs (MXFP4 200 x 1024 x 8192: 6 splits
-// 7.8 us, 8 splits 9.1; FP8 12.4 and 18.6).
+// 7.8 us, 8 splits 9.4).
 constexpr int kLongShare = 8;
 int choose_splits(int units, int k_stages, int sm_count, int ctas_per_sm, int most) {
   auto within = [](int s, int limit) { return s < limit ? s : limit; };
@@ -767,7 +770,12 @@ void few_info(int tn, bb_lowp_info* info) {
   switch (tn) {
     case 16: set(FewCfg<kKind, 16>{}); break;
     case 32: set(FewCfg<kKind, 32>{}); break;
-    case 64: set(FewCfg<kKind, 64>{}); break;
+    case 64:
+      if constexpr (is_fp4(kKind)) {
+        set(FewCfg<kKind, 64>{});
+        break;
+      }
+      [[fallthrough]];
     default: set(FewCfg<kKind, 128>{}); break;
   }
 }
@@ -877,14 +885,16 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
     const int k_stages = static_cast<int>((row_bytes + ROW_BYTES - 1) / ROW_BYTES);
     h->few = use_few(m, rb_n, dev.sm_count);
     if (h->few) {
-      h->tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+      // The narrowest tile that holds the tokens; FP8 goes from 32 to the turned
+      // 128 (64 x 8192 x 8192 17.5 us, tiles of 64 18.4; 61 x 5000 x 2896 8.9 and 9.5).
+      h->tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 && !fp8 ? 64 : 128;
       FewParams& p = h->fp;
       p.m = static_cast<int32_t>(m);
       p.n = static_cast<int32_t>(n);
       p.k_stages = k_stages;
       const int units = static_cast<int>(rb_n * (m > h->tn ? (m + h->tn - 1) / h->tn : 1));
       p.tiles_n = static_cast<int32_t>(rb_n);
-      p.splits = choose_splits(units, k_stages, dev.sm_count, fp8 && h->tn > 64 ? 1 : 2, h->tn > 32 ? 6 : kMaxSplits);
+      p.splits = choose_splits(units, k_stages, dev.sm_count, fp8 && h->tn == 128 ? 1 : 2, h->tn > 32 ? 6 : kMaxSplits);
       p.owned = (128 + p.splits - 1) / p.splits;
       p.sfa = static_cast<const float*>(sfa);
       p.sfb = static_cast<const float*>(sfb);
