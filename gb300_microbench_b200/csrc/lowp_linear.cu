@@ -26,8 +26,8 @@ constexpr int kMaxSplits = 8;  // the portable cluster size
 // depend on timing. Tiles of 128 tokens leave the sums in shared memory and
 // read them instead, each CTA some of the tokens (MXFP4 128 x 4096 x 4096 in 4
 // splits 8.4 us read, 9.9 sent; up to 64 tokens sending is faster: NVFP4
-// 64 x 8192 x 8192 12.6 against 12.8, FP8 18.0 against 20.0, and one token 2.4
-// against 3.2 for the smallest launch).
+// 64 x 8192 x 8192 12.6 against 12.8, and one token 2.4 against 3.2 for the
+// smallest launch).
 //
 // FP8: the K blocks' FP32 scales are applied as in the tile kernel, each
 // block accumulated alone in one of BUFS TMEM buffers and promoted by the
@@ -39,15 +39,18 @@ constexpr int kMaxSplits = 8;  // the portable cluster size
 // the operand traffic (256 x 8192 x 8192: 37 us before, 29 after).
 //
 // What bounds it is the weight stream, and then the ends of the launch: two
-// CTAs of up to 113 KiB share an SM (TN <= 128), so about 200 KiB of weights
-// per SM are in flight, and CTAs of the next launch start beside the last
-// ones of this, set up, and fetch their first weights into L2.
+// CTAs of up to 113 KiB share an SM (all but the turned tiles), so about 200 KiB
+// of weights per SM are in flight, and CTAs of the next launch start beside the
+// last ones of this, set up, and fetch their first weights into L2. (A load
+// balanced to the row, by tiles of 97 instead of 128 weight rows and so two
+// CTAs on every SM, was slower: FP8 1 x 14336 x 4096 14.3 us against 13.0. It
+// leaves no place for the next launch.)
 template <int kKind, int kTN>
 struct FewCfg {
   static constexpr int TN = kTN;
   static constexpr bool FP4 = is_fp4(kKind);
   static constexpr bool TURNED = !FP4 && TN == 128;  // tokens on M
-  static constexpr int CTAS_PER_SM = FP4 || TN <= 32 ? 2 : 1;  // FP8's 64 accumulators a thread want a whole SM's registers
+  static constexpr int CTAS_PER_SM = TURNED ? 1 : 2;  // 64 accumulators a thread want a whole SM's registers
   static constexpr int EPI_W = TN <= 32 ? 4 : 8;  // epilogue warps: lane quarters x column halves
   static constexpr int THREADS = 64 + 32 * EPI_W;
   static constexpr int COLS = TN * 4 / EPI_W;     // accumulator columns per epilogue thread
