@@ -295,18 +295,10 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_fp8_kernel(const NormPara
       if (cg >= p.cols) continue;
       const float s = amax == 0.f ? 1.f : __fdiv_rn(amax, kE4m3Max);
       if (lane % kLanes == 0) p.scales[(cg / 128) * p.s_ld + row] = s;
-      // y itself is rounded four times, so a product with the rounded
-      // reciprocal is as good as a rounded quotient here, at a third of the
-      // instructions; a scale whose reciprocal is out of range divides.
-      if (s > 0x1p-60f && s < 0x1p60f) {
-        const float inv = __fdiv_rn(1.f, s);
-        const F2 inv2 = pack2(inv, inv);
-#pragma unroll
-        for (int i = 0; i < kPer; i += 2) unpack2(mul2(pack2(yg[i], yg[i + 1]), inv2), yg[i], yg[i + 1]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) yg[i] = __fdiv_rn(yg[i], s);
-      }
+      // Rounded quotients here too: a product with the rounded reciprocal moves
+      // two to four times as many values across a border of the E4M3 grid as
+      // y's own roundings do (and saves 3 % at the power cap).
+      divide(yg, s, amax);
     }
     if (!has) continue;
     union {
