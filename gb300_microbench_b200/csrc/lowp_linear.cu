@@ -36,7 +36,9 @@ constexpr int kMaxSplits = 8;  // the portable cluster size
 // FP8 tiles of 128 tokens turn the product round (tokens on M, weights on N):
 // a lane then holds one token, so a K block has one scale per lane instead of
 // one per column, whose 64 shared-memory broadcasts per warp stood in the way of
-// the operand traffic (256 x 8192 x 8192: 37 us before, 29 after).
+// the operand traffic (256 x 8192 x 8192: 37 us before, 28.4 after). 4-bit tiles
+// gain nothing by it (MXFP4 256 x 8192 x 8192 15.6 us, 15.4 turned; 200 x 5000 x
+// 2880 8.8 and 10.2): their scales are the tensor core's.
 //
 // What bounds it is the weight stream, and then the ends of the launch: two
 // CTAs of up to 113 KiB share an SM (all but the turned tiles), so about 200 KiB
@@ -557,6 +559,14 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
       const int count = min(C::TN, p.m - m0);
       const uint32_t base = smem_u32(sums) + lane * 16;
       const int n4 = n_blk * 128 + lane * 4;
+      if (C::TURNED && p.splits == 1) {  // all in this CTA's own shared memory
+#pragma unroll 4
+        for (int c = warp - 2; c < count; c += C::EPI_W) {
+          const float4 f = *reinterpret_cast<const float4*>(sums + c * C::PITCH + lane * 4);
+          const float out[4] = {f.x * scale, f.y * scale, f.z * scale, f.w * scale};
+          store_four(p, (m0 + c) * p.ldd + n4, min(4, p.n - n4), out);
+        }
+      } else
       for (int c = rank + (warp - 2) * p.splits; c < count; c += p.splits * C::EPI_W * kBatch) {
         float4 v[kBatch][kMaxSplits];
 #pragma unroll
