@@ -333,13 +333,18 @@ struct Fp4Params {
   uint8_t* data;           // rows x cols / 2
   uint8_t* atoms;
   void* values;            // dequantised values, may be null
-  uint32_t* maxima;        // NVFP4 with a scale to be found: the CTAs' maxima, or null
+  uint32_t* maxima;        // NVFP4 with a scale found by a launch of its own: the CTAs' maxima, or null
   unsigned* finished;      // CTAs that wrote theirs, 0 between launches
   float tensor_scale;      // NVFP4 with a given scale
   float* tensor_scale_out;
 };
 
 constexpr int kFp4Threads = 256;
+// Vectors of x per thread up to which a CTA of the quantising launch finds the
+// tensor scale by itself, in us against a launch of its own: BF16 1 x 4096 (one
+// vector) 1.84 / 4.61, 4 x 4096 2.77 / 4.61, 8 x 4096 3.97 / 4.70, 12 x 4096
+// 5.14 / 4.62; FP32 4 x 4096 (8 vectors) 3.56 / 4.96, 6 x 4096 4.47 / 4.89.
+constexpr int64_t kFindInside = 8;
 constexpr int kMaxPartials = 1184;  // CTAs of the maximum's kernel
 
 // E2M1 codes of 8 values, element i in nibble i; the sign of a zero is dropped.
@@ -421,32 +426,42 @@ __device__ __forceinline__ void put(T* p, const Vec<T>& v) {
   }
 }
 
-// The tensor scale of NVFP4: maxima of |x| over ranges of the tensor, one per
-// CTA; the CTA that finishes last takes the maximum of all and writes the
-// scale, so the quantising launch reads one word. (Bit patterns of
-// non-negative floats order like the floats, a NaN above all.)
+// Maxima of |x| as bit patterns (those of non-negative floats order like the
+// floats, a NaN above all): over a thread's part of the rows first, first +
+// step, ..., and over a block.
+template <typename T, bool kWide>
+__device__ __forceinline__ uint32_t rows_max(const Fp4Params& p, int64_t first, int64_t step) {
+  const int vecs = p.cols / kVE<T>;  // cols % 32 == 0
+  uint32_t m = 0;
+  for (int64_t row = first; row < p.rows; row += step) {
+    const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
+#pragma unroll 4
+    for (int v = threadIdx.x; v < vecs; v += kFp4Threads)
+      m = max(m, __float_as_uint(absmax(get<kWide>(x + v * kVE<T>))) & 0x7fffffffu);
+  }
+  return m;
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* warp_max) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = v;
+  __syncthreads();
+  for (int i = 0; i < kFp4Threads / 32; ++i) v = max(v, warp_max[i]);
+  return v;
+}
+__device__ __forceinline__ float scale_of_max(uint32_t m) {
+  const float g = __fdiv_rn(__uint_as_float(m), kE4m3Max * kE2m1Max);
+  return g > 0.f ? g : 1.f;  // no data, data below 2688 times the least FP32 number, or NaN
+}
+
+// The tensor scale of NVFP4: a maximum per CTA; the CTA that finishes last takes
+// the maximum of all and writes the scale, so the quantising launch reads one word.
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(kFp4Threads) absmax_kernel(const Fp4Params p) {
   __shared__ uint32_t warp_max[kFp4Threads / 32];
   __shared__ bool last;
   grid_wait();
   grid_trigger();
-  const int vecs = p.cols / kVE<T>;  // cols % 32 == 0
-  uint32_t m = 0;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
-#pragma unroll 2
-    for (int v = threadIdx.x; v < vecs; v += blockDim.x)
-      m = max(m, __float_as_uint(absmax(get<kWide>(x + v * kVE<T>))) & 0x7fffffffu);
-  }
-  auto block_max = [&](uint32_t v) {
-    v = __reduce_max_sync(0xffffffffu, v);
-    if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = v;
-    __syncthreads();
-    for (int i = 0; i < kFp4Threads / 32; ++i) v = max(v, warp_max[i]);
-    return v;
-  };
-  m = block_max(m);
+  uint32_t m = block_max(rows_max<T, kWide>(p, blockIdx.x, gridDim.x), warp_max);
   if (threadIdx.x == 0) {
     p.maxima[blockIdx.x] = m;
     __threadfence();
@@ -457,11 +472,8 @@ __global__ void __launch_bounds__(kFp4Threads) absmax_kernel(const Fp4Params p) 
   __threadfence();
   m = 0;
   for (unsigned i = threadIdx.x; i < gridDim.x; i += blockDim.x) m = max(m, __ldcg(p.maxima + i));
-  m = block_max(m);
-  if (threadIdx.x == 0) {
-    const float g = __fdiv_rn(__uint_as_float(m), kE4m3Max * kE2m1Max);
-    *p.tensor_scale_out = g > 0.f ? g : 1.f;  // no data, data below 2688 times the least FP32 number, or NaN
-  }
+  m = block_max(m, warp_max);
+  if (threadIdx.x == 0) *p.tensor_scale_out = scale_of_max(m);
 }
 
 // A thread owns 16 columns of a row: one NVFP4 block, or half an MXFP4 block
@@ -473,7 +485,13 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quant_kernel(const Fp4Params 
   grid_trigger();
   float g = p.tensor_scale;
   if constexpr (!kMx) {
-    if (p.maxima) g = *p.tensor_scale_out;
+    if (p.maxima) {
+      g = *p.tensor_scale_out;
+    } else if (p.tensor_scale_out) {  // a small tensor: every CTA reads all of it
+      __shared__ uint32_t warp_max[kFp4Threads / 32];
+      g = scale_of_max(block_max(rows_max<T, kWide>(p, 0, 1), warp_max));
+      if (blockIdx.x == 0 && threadIdx.x == 0) *p.tensor_scale_out = g;
+    }
   }
   constexpr int kLanes = kMx ? 8 : 4;  // threads of one row's part of an atom
   const uint32_t per_row = static_cast<uint32_t>(p.atoms_k) * kLanes;
@@ -712,7 +730,11 @@ BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, cons
     p.values = values;
     p.tensor_scale = tensor_scale;
     p.tensor_scale_out = tensor_scale_out;
-    if (find && rows > 0) {
+    // A small tensor's scale is found by every CTA of the quantising launch
+    // itself, a larger one's by a launch of its own; also where `values` is
+    // written, which may be x: a CTA would overwrite what another still reads.
+    const int64_t per_thread = (cols * static_cast<int64_t>(size) / 32 + kFp4Threads - 1) / kFp4Threads;
+    if (find && rows > 0 && (values || rows * per_thread > kFindInside)) {
       const int64_t most = 8ll * dev.sm_count < kMaxPartials ? 8ll * dev.sm_count : kMaxPartials;
       h->partials = static_cast<int>(rows < most ? rows : most);
       const size_t bytes = (h->partials + 1) * sizeof(uint32_t);

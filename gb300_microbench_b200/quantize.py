@@ -130,7 +130,8 @@ class Fp4QuantPlan(_QuantPlan):
     :class:`.lowp.Nvfp4Operand` or :class:`.lowp.Mxfp4Operand` made by its
     ``empty``: codes, and scales as the atoms the product reads. An NVFP4
     operand without a tensor scale has it found from x at every run (one more
-    launch and reading of x) and left in ``out.tensor_scale_out``.
+    reading of x, and one more launch unless x is a few rows and ``values`` is
+    not given) and left in ``out.tensor_scale_out``.
 
     ``values``, if given, is (rows, K) of x's dtype and receives what the codes
     stand for (x as the product sees it: the forward value of

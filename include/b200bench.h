@@ -340,8 +340,9 @@ typedef struct bb_quant_plan bb_quant_plan;
  * BB_LOWP_MXFP4: E2M1 codes into data (rows x cols / 2 bytes) and scale atoms
  * (padding rows and columns zero) into scales, as bb_linear_plan_create reads
  * them. NVFP4 with tensor_scale_out == NULL uses tensor_scale; otherwise the
- * tensor scale is max|x| / 2688 (1 where that is 0 in FP32 or NaN), found by a launch of its
- * own and written to *tensor_scale_out (device). values (may be NULL, x's
+ * tensor scale is max|x| / 2688 (1 where that is 0 in FP32 or NaN), found at
+ * every run (by a launch of its own unless the tensor is a few rows) and written to
+ * *tensor_scale_out (device). values (may be NULL, x's
  * dtype, row stride values_ld) receives what the codes stand for. */
 BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t x_ld,
                                     void* data, void* scales, float tensor_scale, float* tensor_scale_out,

@@ -243,6 +243,42 @@ def test_fp4_strides_and_in_place(cuda_device, fmt, shift):
     assert torch.equal(full[:, :shift], keep[:, :shift]) and torch.equal(full[:, shift + 96:], keep[:, shift + 96:])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1, 32), (1, 4096), (1, 16384), (1, 32800), (3, 4096), (8, 512), (9, 512), (5, 2880)])
+@pytest.mark.parametrize("shift", [0, 3])
+def test_fp4_found_scale_of_few_rows(cuda_device, dtype, rows, k, shift):
+    """The scale of a few rows, found with and without a launch of its own: the maximum in the last row's
+    last block, no values, then values over x itself (no CTA may read x after another wrote it)."""
+    full = torch.zeros(rows, k + 16, dtype=dtype, device=cuda_device)
+    x = full[:, shift:shift + k]
+    x.copy_(_x(rows, k, dtype, seed=rows + k).to(cuda_device))
+    x[-1, -1] = -900.0
+    packed, bits, g, deq = _fp4_reference("nvfp4", x.cpu())
+    atoms = lowp.pack_scale_atoms(bits)
+    for values in (None, x):
+        op = lowp.Nvfp4Operand.empty(rows, k, device=cuda_device)
+        plan = quantize.Fp4QuantPlan(x, op, values=values)
+        plan.run()
+        plan.synchronize()
+        assert torch.equal(op.data.cpu(), packed) and torch.equal(op.atoms.cpu(), atoms)
+        assert float(op.tensor_scale_out) == float(torch.tensor(g, dtype=torch.float32))
+        plan.close()
+    assert torch.equal(x.cpu(), deq.to(dtype))
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("fill", [0.0, float("nan"), float("inf"), 1e-40])
+def test_fp4_found_scale_without_a_maximum(cuda_device, rows, fill):
+    """Zero, NaN, an infinity and data below 2688 times the least FP32 number, the same for a few rows and many."""
+    x = torch.zeros(rows, 512)
+    x[rows // 2, 40] = fill
+    packed, bits, g, _ = _fp4_reference("nvfp4", x)
+    op, _ = _fp4("nvfp4", x, cuda_device, values=False)
+    # inf / inf is a NaN whose sign IEEE 754 leaves open, 0x7f or 0xff in E4M3; the kernel writes 0x7f.
+    assert torch.equal(op.data, packed) and torch.equal(op.atoms, lowp.pack_scale_atoms(bits & 0x7F))
+    assert float(op.tensor_scale_out) == float(torch.tensor(g, dtype=torch.float32))
+
+
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 def test_fp4_no_rows(cuda_device, fmt):
     op, v = _fp4(fmt, torch.empty(0, 64, dtype=torch.bfloat16), cuda_device)
