@@ -55,7 +55,7 @@ struct DeviceInfo {
 };
 int query_device(DeviceInfo* info);
 
-// Makes the plan's device current for a launch, and the caller's again after it.
+// Makes the plan's device current for a launch or a wait, and the caller's again after it.
 struct DeviceGuard {
   int before = -1;
   cudaError_t status;
@@ -68,5 +68,15 @@ struct DeviceGuard {
     if (before >= 0) cudaSetDevice(before);
   }
 };
+
+// Zeroed device memory that a launch on any stream may use next: cudaMemset
+// runs on the default stream, behind what is queued there, and streams that do
+// not synchronise with it would not wait for it.
+inline int device_zeros(void** p, size_t bytes, const char* what) {
+  int rc = check_cuda(cudaMalloc(p, bytes), what);
+  if (rc == BB_OK) rc = check_cuda(cudaMemset(*p, 0, bytes), what);
+  if (rc == BB_OK) rc = check_cuda(cudaStreamSynchronize(nullptr), what);
+  return rc;
+}
 
 }  // namespace bb

@@ -976,8 +976,7 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
         rc = encode_tiled(&h->tm_d, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 2, d, dims, strides, box,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
       }
-      if (rc == BB_OK) rc = check_cuda(cudaMalloc(&h->status_dev, sizeof(int)), "cudaMalloc(status)");
-      if (rc == BB_OK) rc = check_cuda(cudaMemset(h->status_dev, 0, sizeof(int)), "cudaMemset(status)");
+      if (rc == BB_OK) rc = device_zeros(reinterpret_cast<void**>(&h->status_dev), sizeof(int), "allocation of the status word");
       if (rc != BB_OK) {
         if (h->status_dev) cudaFree(h->status_dev);
         delete h;
@@ -1043,6 +1042,8 @@ BB_API int bb_linear_synchronize(bb_linear_plan* plan) {
       set_error("bb_linear_synchronize: null plan");
       return BB_ERR_ARGUMENT;
     }
+    DeviceGuard guard(plan->device);  // the default stream is the current device's
+    BB_CUDA_TRY(guard.status);
     BB_CUDA_TRY(cudaStreamSynchronize(plan->stream));
     if (!plan->status_dev) return BB_OK;
     int st = 0;

@@ -738,8 +738,7 @@ BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, cons
       const int64_t most = 8ll * dev.sm_count < kMaxPartials ? 8ll * dev.sm_count : kMaxPartials;
       h->partials = static_cast<int>(rows < most ? rows : most);
       const size_t bytes = (h->partials + 1) * sizeof(uint32_t);
-      rc = check_cuda(cudaMalloc(&p.maxima, bytes), "cudaMalloc(maxima)");
-      if (rc == BB_OK) rc = check_cuda(cudaMemset(p.maxima, 0, bytes), "cudaMemset(maxima)");
+      rc = device_zeros(reinterpret_cast<void**>(&p.maxima), bytes, "allocation of the maxima");
       if (rc != BB_OK) {
         if (p.maxima) cudaFree(p.maxima);
         delete h;
@@ -879,6 +878,8 @@ BB_API int bb_quant_synchronize(bb_quant_plan* plan) {
     set_error("bb_quant_synchronize: null plan");
     return BB_ERR_ARGUMENT;
   }
+  DeviceGuard guard(plan->device);  // the default stream is the current device's
+  if (guard.status != cudaSuccess) return check_cuda(guard.status, "cudaSetDevice");
   return check_cuda(cudaStreamSynchronize(plan->stream), "cudaStreamSynchronize");
 }
 

@@ -322,6 +322,27 @@ def test_other_stream_and_graph(cuda_device):
         assert float(nv.tensor_scale_out) == float(torch.tensor(g, dtype=torch.float32))
 
 
+def test_plan_made_while_the_default_stream_is_busy(cuda_device):
+    """The counter of the maximum's launch is zero before a plan on another stream first runs, whatever the
+    memory held and whatever is queued on the default stream (a busy wait of about 10 ms)."""
+    big = _x(1184, 64, torch.bfloat16).to(cuda_device)
+    plan = quantize.Fp4QuantPlan(big, lowp.Nvfp4Operand.empty(1184, 64, device=cuda_device))
+    plan.run()
+    plan.synchronize()
+    plan.close()  # its maxima stay behind in the memory that the next plan gets
+    stream = torch.cuda.Stream(device=cuda_device)
+    x = _x(20, 64, torch.bfloat16, seed=3)
+    xd, op = x.to(cuda_device), lowp.Nvfp4Operand.empty(20, 64, device=cuda_device)
+    torch.cuda.synchronize(cuda_device)
+    torch.cuda._sleep(20_000_000)
+    plan = quantize.Fp4QuantPlan(xd, op, stream=stream)
+    plan.run()
+    plan.synchronize()
+    packed, bits, g, _ = _fp4_reference("nvfp4", x)
+    assert torch.equal(op.data.cpu(), packed) and torch.equal(op.atoms.cpu(), lowp.pack_scale_atoms(bits))
+    assert float(op.tensor_scale_out) == float(torch.tensor(g, dtype=torch.float32))
+
+
 def test_row_strides_past_32_bits(cuda_device):
     """Rows 2^31 elements apart."""
     ld, cols = 1 << 31, 288
