@@ -684,6 +684,42 @@ int launch_few_kind(const bb_linear_plan& pl) {
   }
 }
 
+// Clusters of `splits` CTAs that are resident at once: fewer than the SMs would
+// hold of single CTAs, since a cluster's SMs are neighbours (148 SMs hold 74, 45,
+// 33, 26, 22, 15 and 15 clusters of 2 to 8 CTAs). The query counts one CTA per SM.
+// Asked once per kernel, device and size.
+template <int kKind, int kTN>
+int resident_clusters(int device, int sm_count, int splits, int* clusters) {
+  using C = FewCfg<kKind, kTN>;
+  static bool done[kMaxDevices] = {};
+  static int known[kMaxDevices][kMaxSplits + 1] = {};
+  if (device < kMaxDevices && known[device][splits]) {
+    *clusters = known[device][splits];
+    return BB_OK;
+  }
+  auto kernel = few_rows_kernel<kKind, kTN>;
+  int rc = allow_smem(kernel, C::SMEM_BYTES, device, done);
+  if (rc != BB_OK) return rc;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = config(sm_count / splits * splits, C::THREADS, C::SMEM_BYTES, splits, false, nullptr, attr);
+  BB_CUDA_TRY(cudaOccupancyMaxActiveClusters(clusters, kernel, &cfg));
+  *clusters *= C::CTAS_PER_SM;
+  if (device < kMaxDevices) known[device][splits] = *clusters;
+  return BB_OK;
+}
+
+template <int kKind>
+int resident_clusters_of(int tn, int device, int sm_count, int splits, int* clusters) {
+  switch (tn) {
+    case 16: return resident_clusters<kKind, 16>(device, sm_count, splits, clusters);
+    case 32: return resident_clusters<kKind, 32>(device, sm_count, splits, clusters);
+    case 64:
+      if constexpr (is_fp4(kKind)) return resident_clusters<kKind, 64>(device, sm_count, splits, clusters);
+      [[fallthrough]];
+    default: return resident_clusters<kKind, 128>(device, sm_count, splits, clusters);
+  }
+}
+
 template <int kKind, int kCG, bool kDirect>
 int launch_tile(const bb_linear_plan& pl) {
   using C = Cfg<kKind, kCG>;
@@ -759,16 +795,50 @@ bool use_few(int64_t m, int64_t rb_n, int sm_count) { return m <= 128 || rb_n * 
 // weight stream in flight (NVFP4 1 x 8192 x 8192: 2 splits 10.4 us, 4 splits
 // 8.6; FP8 1 x 14336 x 4096: 1 split 14.4, 2 splits 12.9) where each still has
 // kLongShare stages. Never more CTAs than are resident at once: a second wave
-// costs half the kernel (6 splits of the same NVFP4 case 12.0 us). Sums of
+// costs half the kernel (6 splits of the same NVFP4 case 12.0 us; FP8 512 x 768 x
+// 1536, 24 tiles at one CTA per SM, of which 22 clusters of 6 fit: 13.5 us, 7.5 with 5 splits). Sums of
 // many tokens are read from at most six CTAs (MXFP4 200 x 1024 x 8192: 6 splits
 // 7.8 us, 8 splits 9.4).
 constexpr int kLongShare = 8;
-int choose_splits(int units, int k_stages, int sm_count, int ctas_per_sm, int most) {
-  auto within = [](int s, int limit) { return s < limit ? s : limit; };
-  int s = within(within(sm_count / units, most), k_stages / 2);
-  const int more = within(within(sm_count * ctas_per_sm / units, most), k_stages / kLongShare);
-  if (more > s) s = more;
-  return s < 1 ? 1 : s;
+int choose_splits(int kind, int tn, int64_t units, int k_stages, const DeviceInfo& dev, int* splits) {
+  const int ctas_per_sm = kind == BB_LOWP_FP8_GROUP128 && tn == 128 ? 1 : 2, most = tn > 32 ? 6 : kMaxSplits;
+  // The largest number of splits up to `limit` whose clusters are all resident.
+  auto fitting = [&](int64_t limit, int* s) -> int {
+    *s = static_cast<int>(limit < most ? limit : most);
+    for (; *s > 1; --*s) {
+      int clusters = 0;
+      const int rc = kind == BB_LOWP_NVFP4   ? resident_clusters_of<kNvfp4>(tn, dev.device, dev.sm_count, *s, &clusters)
+                     : kind == BB_LOWP_MXFP4 ? resident_clusters_of<kMxfp4>(tn, dev.device, dev.sm_count, *s, &clusters)
+                                             : resident_clusters_of<kFp8Group>(tn, dev.device, dev.sm_count, *s, &clusters);
+      if (rc != BB_OK) return rc;
+      if (units <= clusters) return BB_OK;
+    }
+    *s = 1;
+    return BB_OK;
+  };
+  auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
+  int one = 1, two = 1;
+  int rc = fitting(least(dev.sm_count / units, k_stages / 2), &one);
+  if (rc == BB_OK) rc = fitting(least(dev.sm_count * ctas_per_sm / units, k_stages / kLongShare), &two);
+  *splits = one > two ? one : two;
+  return rc;
+}
+
+// Estimated us of the FP8 few-rows kernel with tiles of tn tokens: the launch and
+// its ends, the exchange of split sums, a time per K block of a CTA (half as much
+// again where two CTAs share an SM) and the operand traffic from L2. Fitted to 518
+// shapes (K 256 to 13584, N 64 to 5000, M 24 to 2048, FP8 weights in L2): what it
+// chooses takes 0.6 % longer than the best of the three on average (19 % at worst),
+// and 18 % less than tiles of 128 always: N x K = 256 x 4096, M = 200: tiles of
+// 128 / 32 / 16 7.7 / 4.8 / 5.0 us; 512 x 640, 128: 6.2 / 4.7 / 3.8; 5000 x 2896, 64:
+// 8.2 / 10.2 / 12.4; 4096 x 13584, 128: 18.4 / 37 / 57.
+float fp8_few_time(int tn, int64_t m, int64_t units, int k_stages, int splits, int sm_count) {
+  const int64_t ctas = units * splits, places = sm_count * (tn == 128 ? 1 : 2);
+  const int64_t waves = (ctas + places - 1) / places;
+  const float start = (tn == 128 ? 3.0f + 0.02f * (m < 128 ? m : 128) : tn == 32 ? 3.0f : 2.5f) + (splits > 1 ? 0.6f : 0.f);
+  const float block = tn == 128 ? 0.30f : (tn == 32 ? 0.27f : 0.25f) * (ctas > sm_count ? 1.5f : 1.f);
+  const float mbytes = units * k_stages * (128 + tn) * ROW_BYTES * 1e-6f;
+  return start * (1 + 0.5f * (waves - 1)) + waves * (static_cast<float>(k_stages) / splits) * block + mbytes / 30.f;
 }
 
 template <int kKind>
@@ -898,16 +968,38 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
     const int k_stages = static_cast<int>((row_bytes + ROW_BYTES - 1) / ROW_BYTES);
     h->few = use_few(m, rb_n, dev.sm_count);
     if (h->few) {
-      // The narrowest tile that holds the tokens; FP8 goes from 32 to the turned
-      // 128 (64 x 8192 x 8192 17.5 us, tiles of 64 18.4; 61 x 5000 x 2896 8.9 and 9.5).
-      h->tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 && !fp8 ? 64 : 128;
+      // 4-bit: the narrowest tile that holds the tokens (a tile below 128 tokens
+      // cannot start inside a 128-row scale block). FP8: what is estimated
+      // fastest, of 64 tokens never (64 x 8192 x 8192: 18.4 us, the turned tiles
+      // of 128 17.5; 61 x 5000 x 2896 9.5 and 8.9).
       FewParams& p = h->fp;
+      if (!fp8) {
+        h->tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+        rc = choose_splits(kind, h->tn, rb_n * (rb_m > 1 ? rb_m : 1), k_stages, dev, &p.splits);
+      } else {
+        float least = 0.f;
+        for (int tn = 16; tn <= 128 && rc == BB_OK; tn = tn == 16 ? 32 : tn * 4) {
+          const int64_t units = rb_n * (m > tn ? (m + tn - 1) / tn : 1);
+          int splits = 1;
+          rc = choose_splits(kind, tn, units, k_stages, dev, &splits);
+          const float t = fp8_few_time(tn, m, units, k_stages, splits, dev.sm_count);
+          if (tn == 16 || t < least) {
+            least = t;
+            h->tn = tn;
+            p.splits = splits;
+          }
+          if (tn >= m) break;  // a wider tile holds no more
+        }
+      }
+      if (rc != BB_OK) {
+        delete h;
+        return rc;
+      }
       p.m = static_cast<int32_t>(m);
       p.n = static_cast<int32_t>(n);
       p.k_stages = k_stages;
       const int units = static_cast<int>(rb_n * (m > h->tn ? (m + h->tn - 1) / h->tn : 1));
       p.tiles_n = static_cast<int32_t>(rb_n);
-      p.splits = choose_splits(units, k_stages, dev.sm_count, fp8 && h->tn == 128 ? 1 : 2, h->tn > 32 ? 6 : kMaxSplits);
       p.owned = (128 + p.splits - 1) / p.splits;
       p.sfa = static_cast<const float*>(sfa);
       p.sfb = static_cast<const float*>(sfb);

@@ -106,6 +106,25 @@ def test_exact_widths(cuda_device, kind, m, n):
     assert torch.equal(_run(x, w, cuda_device), want.float().to(torch.bfloat16))
 
 
+# Token tiles of the FP8 kernel for few rows, with and without K split: several tiles of 16 or 32 tokens,
+# the last one with a single token, and 128 tokens.
+@pytest.mark.parametrize("m,n,k,tile,split", [
+    (17, 264, 544, 16, True), (129, 1000, 288, 16, False), (100, 264, 1040, 16, True), (513, 264, 528, 16, False),
+    (257, 140, 4096, 32, True), (193, 777, 1056, 32, True), (1281, 264, 528, 32, False), (65, 12000, 528, 32, False),
+    (513, 640, 2048, 128, True), (600, 1100, 4096, 128, True), (300, 6000, 528, 128, False), (1000, 500, 8192, 128, True)])
+def test_exact_fp8_tiles(cuda_device, m, n, k, tile, split):
+    gen = torch.Generator().manual_seed(m)
+    x, w = _exact_operand("fp8", m, k, gen, False), _exact_operand("fp8", n, k, gen, True)
+    want = _decode(x) @ _decode(w).T
+    d = torch.full((m + 2, n + 3), 7.0, device=cuda_device)
+    plan = lowp.LowpLinearPlan(x.to(cuda_device), w.to(cuda_device), d[:m, :n])
+    assert plan.info["few_rows"] and plan.info["tile_m"] == tile and (plan.info["k_splits"] > 1) == split
+    plan.run(3)
+    plan.synchronize()
+    assert torch.equal(d[:m, :n].cpu().double(), want)
+    assert (d[m:] == 7).all() and (d[:, n:] == 7).all()
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("m", [1, 24, 257])
 @pytest.mark.parametrize("k", [16, 32, 64, 96, 128, 144, 160, 256, 272, 512, 1040, 2880, 4096])
