@@ -841,6 +841,23 @@ float fp8_few_time(int tn, int64_t m, int64_t units, int k_stages, int splits, i
   return start * (1 + 0.5f * (waves - 1)) + waves * (static_cast<float>(k_stages) / splits) * block + mbytes / 30.f;
 }
 
+// Estimated us of the tile kernel with tiles of a CTA pair (256 x 256) or of one
+// CTA (128 x 256), in waves of the tiles that are resident at once, without what
+// both have. A pair reads half of B per CTA and ends later; its tiles leave more
+// of the last wave and of the rows below M empty. FP8 is bound by the promotion
+// either way (us, pairs / single: 1453 x 2560 x 768 8.2 / 7.2, 526 x 12720 x 2240,
+// 3 waves against 2, 31 / 23, 2537 x 12720 x 8192 equal); 4-bit tiles by the
+// operands (1100 x 2560 x 768 6.6 / 6.0, 526 x 12720 x 768 9.6 / 8.0, x 2240 15.0 /
+// 14.3, 1100 x 5120 x 2240 12.2 / 14.0, x 8192 25.8 / 35.2). Where rows do not begin
+// on a 32-byte sector, every box of a row is one sector more, and single CTAs are
+// bound by the operands sooner (FP8 1453 x 7680 x 1232 23.5 / 27.7, 7765 x 3200 x 528
+// 29.2 / 32.3).
+float tile_time(bool fp8, int cg, int64_t waves, int k_stages, bool sectors) {
+  const float end = cg == 1 ? 0.f : fp8 ? 0.9f : 0.7f;
+  const float stage = fp8 ? (cg == 2 ? 0.5f : 0.505f) : (cg == 2 ? 0.33f : 0.48f);
+  return end + static_cast<float>(waves * k_stages) * stage * (cg == 1 && !sectors ? 1.3f : 1.f);
+}
+
 template <int kKind>
 void few_info(int tn, bb_lowp_info* info) {
   auto set = [&](auto cfg) {
@@ -1012,28 +1029,34 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
       p.d_dtype = d_dtype;
       h->grid = units * p.splits;
     } else {
-      h->cg = 2;
+      int pairs = 0;
+      rc = kind == kNvfp4   ? resident_pairs<kNvfp4>(*h, dev.sm_count, &pairs)
+           : kind == kMxfp4 ? resident_pairs<kMxfp4>(*h, dev.sm_count, &pairs)
+                            : resident_pairs<kFp8Group>(*h, dev.sm_count, &pairs);
+      if (rc != BB_OK) {
+        delete h;
+        return rc;
+      }
+      const int64_t tiles_n = (n + 255) / 256;
+      auto time = [&](int cg, int64_t resident) {
+        const int64_t tiles = (m + BM * cg - 1) / (BM * cg) * tiles_n;
+        return tile_time(fp8, cg, (tiles + resident - 1) / resident, k_stages, row_bytes % 32 == 0);
+      };
+      h->cg = time(1, dev.sm_count) < time(2, pairs) ? 1 : 2;
+      const int clusters = h->cg == 2 ? pairs : dev.sm_count;
       Params& p = h->tile;
       const int tile_m = BM * h->cg;
       p.m = static_cast<int32_t>(m);
       p.n = static_cast<int32_t>(n);
       p.k = static_cast<int32_t>(k);
       p.tiles_m = static_cast<int32_t>((m + tile_m - 1) / tile_m);
-      p.tiles_n = static_cast<int32_t>((n + 255) / 256);
+      p.tiles_n = static_cast<int32_t>(tiles_n);
       p.num_tiles = p.tiles_m * p.tiles_n;
       p.k_stages = k_stages;
       p.rb_m = static_cast<int32_t>(rb_m);
       p.rb_n = static_cast<int32_t>(rb_n);
       const int64_t g = kGroupABytes / (tile_m * row_bytes);
       p.group_m = static_cast<int32_t>(g < 1 ? 1 : g > p.tiles_m ? p.tiles_m : g);
-      int clusters = 0;
-      rc = kind == kNvfp4   ? resident_pairs<kNvfp4>(*h, dev.sm_count, &clusters)
-           : kind == kMxfp4 ? resident_pairs<kMxfp4>(*h, dev.sm_count, &clusters)
-                            : resident_pairs<kFp8Group>(*h, dev.sm_count, &clusters);
-      if (rc != BB_OK) {
-        delete h;
-        return rc;
-      }
       p.num_clusters = p.num_tiles < clusters ? p.num_tiles : clusters;
       p.sfa = static_cast<const uint8_t*>(sfa);
       p.sfb = static_cast<const uint8_t*>(sfb);

@@ -199,6 +199,27 @@ def test_many_tiles_strided_output(cuda_device, kind, dtype, pad, shift):
     assert torch.equal(full.cpu(), want)
 
 
+# Three waves of 256 x 256 tiles and a long K: CTA pairs for every kind; a few K: one CTA per tile.
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n,k,pad,dtype,pairs", [
+    (2300, 4304, 8192, 0, torch.bfloat16, True), (2300, 4303, 8192, 2, torch.float32, True),
+    (2300, 4301, 8192, 0, torch.float16, True), (1400, 3304, 576, 0, torch.bfloat16, False),
+    (1400, 3303, 576, 2, torch.bfloat16, False), (2304, 4304, 1040, 0, torch.bfloat16, True)])
+def test_tiles_of_pairs_and_single_ctas(cuda_device, kind, m, n, k, pad, dtype, pairs):
+    gen = torch.Generator().manual_seed(n)
+    k = _round_up(k, kind)
+    x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+    rows = torch.cat([torch.arange(0, m, 37), torch.arange(m - 4, m)])
+    want = (_decode(x)[rows].float().to(cuda_device).double() @ _decode(w).float().to(cuda_device).double().T).float()
+    full = torch.full((m, n + pad), -7.0, dtype=dtype, device=cuda_device)
+    plan = lowp.LowpLinearPlan(x.to(cuda_device), w.to(cuda_device), full[:, :n])
+    assert plan.info["few_rows"] == 0 and plan.info["cta_group"] == (2 if pairs else 1)
+    plan.run(2)
+    plan.synchronize()
+    assert torch.equal(full[rows.to(cuda_device), :n], want.to(dtype))
+    assert (full[:, n:] == -7).all()
+
+
 @pytest.mark.parametrize("dtype", list(HALF_STEP))
 @pytest.mark.parametrize("kind", KINDS)
 def test_many_tiles_quantised(cuda_device, kind, dtype):
