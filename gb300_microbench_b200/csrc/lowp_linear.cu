@@ -789,27 +789,24 @@ int launch_linear(const bb_linear_plan& pl) {
 // 33.0 / 20.3, MXFP4 11.6 / 11.4).
 bool use_few(int64_t m, int64_t rb_n, int sm_count) { return m <= 128 || rb_n * ((m + 127) / 128) <= sm_count; }
 
-// K splits of the few-rows kernel. One CTA per SM suffices for a short K: more
-// of them only add to the exchange (MXFP4 128 x 4096 x 4096, 32 row blocks:
-// 4 splits 8.4 us, 8 splits 12.8). A second CTA per SM keeps more of a long
-// weight stream in flight (NVFP4 1 x 8192 x 8192: 2 splits 10.4 us, 4 splits
-// 8.6; FP8 1 x 14336 x 4096: 1 split 14.4, 2 splits 12.9) where each still has
-// kLongShare stages. Never more CTAs than are resident at once: a second wave
-// costs half the kernel (6 splits of the same NVFP4 case 12.0 us; FP8 512 x 768 x
-// 1536, 24 tiles at one CTA per SM, of which 22 clusters of 6 fit: 13.5 us, 7.5 with 5 splits). Sums of
-// many tokens are read from at most six CTAs (MXFP4 200 x 1024 x 8192: 6 splits
-// 7.8 us, 8 splits 9.4).
+// K splits of the few-rows kernel. A split shortens a CTA's stream of K blocks and
+// costs the exchange of the sums; never more CTAs than are resident at once, since
+// a second wave costs half the kernel (NVFP4 1 x 8192 x 8192: 4 splits 8.6 us, 6
+// 12.0; FP8 512 x 768 x 1536, 24 tiles at one CTA per SM, of which 22 clusters of 6
+// fit: 13.5 us, 7.5 with 5 splits).
+//
+// FP8: one CTA per SM suffices for a short K; a second one keeps more of a long
+// weight stream in flight (1 x 14336 x 4096: 1 split 14.4, 2 splits 12.9) where
+// each still has kLongShare blocks. Sums of many tokens are read from at most six CTAs.
 constexpr int kLongShare = 8;
-int choose_splits(int kind, int tn, int64_t units, int k_stages, const DeviceInfo& dev, int* splits) {
-  const int ctas_per_sm = kind == BB_LOWP_FP8_GROUP128 && tn == 128 ? 1 : 2, most = tn > 32 ? 6 : kMaxSplits;
+int fp8_splits(int tn, int64_t units, int k_stages, const DeviceInfo& dev, int* splits) {
+  const int ctas_per_sm = tn == 128 ? 1 : 2, most = tn > 32 ? 6 : kMaxSplits;
   // The largest number of splits up to `limit` whose clusters are all resident.
   auto fitting = [&](int64_t limit, int* s) -> int {
     *s = static_cast<int>(limit < most ? limit : most);
     for (; *s > 1; --*s) {
       int clusters = 0;
-      const int rc = kind == BB_LOWP_NVFP4   ? resident_clusters_of<kNvfp4>(tn, dev.device, dev.sm_count, *s, &clusters)
-                     : kind == BB_LOWP_MXFP4 ? resident_clusters_of<kMxfp4>(tn, dev.device, dev.sm_count, *s, &clusters)
-                                             : resident_clusters_of<kFp8Group>(tn, dev.device, dev.sm_count, *s, &clusters);
+      const int rc = resident_clusters_of<kFp8Group>(tn, dev.device, dev.sm_count, *s, &clusters);
       if (rc != BB_OK) return rc;
       if (units <= clusters) return BB_OK;
     }
@@ -822,6 +819,45 @@ int choose_splits(int kind, int tn, int64_t units, int k_stages, const DeviceInf
   if (rc == BB_OK) rc = fitting(least(dev.sm_count * ctas_per_sm / units, k_stages / kLongShare), &two);
   *splits = one > two ? one : two;
   return rc;
+}
+
+// 4-bit formats: the splits that are estimated fastest, in us: 0.25 to 0.27 per K
+// stage of a CTA, against an exchange whose time depends on the tile's tokens and
+// grows with the CTAs, above all where SMs hold two of them. Fitted to 400 shapes
+// (K 512 to 12288, N 128 to 5000, M 12 to 1100): 0.9 % longer than the best on
+// average (12 % at worst), 6 % less than as many splits as the SMs take. MXFP4 60 x
+// 5000 x 1024: 1 split 3.5, 2 splits 5.6; 60 x 1024 x 8192: 1, 4, 8 splits 10.6, 6.8,
+// 5.8; 500 x 1024 x 12288: 1, 4, 6 splits 16.4, 9.1, 12.8. Where many tokens' tiles
+// leave no choice but one split or shared SMs, a long stream of weights (16 MB and
+// more) is faster through shared SMs (200 x 5000 x 12288: 1 split 21.1, 2 16.2, 3
+// 15.4; 256 x 8192 x 8192, L2 cold: 24.6, 23.3).
+template <int kKind>
+int fp4_splits(int tn, int64_t units, int64_t rb_n, int k_stages, const DeviceInfo& dev, int* splits) {
+  const bool stream = tn == 128 && 2 * units > dev.sm_count && rb_n * k_stages * 128 * ROW_BYTES >= (16 << 20);
+  const float block = tn == 128 ? 0.27f : 0.25f;
+  const float exchange = tn == 16 ? 0.6f : tn == 32 ? 0.8f : tn == 64 ? 2.0f : 1.9f;
+  const float per_cta = (tn == 16 || tn == 32 ? 0.4f : tn == 64 ? 0.5f : 0.6f) / 100;
+  const float shared_sms = tn == 16 ? 0.3f : tn == 32 ? 0.5f : tn == 64 ? 1.3f : stream ? 0.f : 3.0f;
+  const int most = tn == 128 ? 6 : kMaxSplits;
+  float least = 0.f;
+  for (int s = 1; s <= most && s <= k_stages; ++s) {
+    float t = static_cast<float>(k_stages) / s * block * (stream && s == 1 ? 1.3f : 1.f);
+    if (s > 1) {
+      int clusters = 0;
+      const int rc = resident_clusters_of<kKind>(tn, dev.device, dev.sm_count, s, &clusters);
+      if (rc != BB_OK) return rc;
+      if (units > clusters) continue;
+      t += exchange + static_cast<float>(units * s) * per_cta;
+      if (2 * units > clusters) t += shared_sms;
+    } else if (units > dev.sm_count) {
+      t += shared_sms;
+    }
+    if (s == 1 || t < least) {
+      least = t;
+      *splits = s;
+    }
+  }
+  return BB_OK;
 }
 
 // Estimated us of the FP8 few-rows kernel with tiles of tn tokens: the launch and
@@ -992,13 +1028,15 @@ BB_API int bb_linear_plan_create(int kind, int64_t m, int64_t n, int64_t k, cons
       FewParams& p = h->fp;
       if (!fp8) {
         h->tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-        rc = choose_splits(kind, h->tn, rb_n * (rb_m > 1 ? rb_m : 1), k_stages, dev, &p.splits);
+        const int64_t units = rb_n * (rb_m > 1 ? rb_m : 1);
+        rc = kind == kNvfp4 ? fp4_splits<kNvfp4>(h->tn, units, rb_n, k_stages, dev, &p.splits)
+                            : fp4_splits<kMxfp4>(h->tn, units, rb_n, k_stages, dev, &p.splits);
       } else {
         float least = 0.f;
         for (int tn = 16; tn <= 128 && rc == BB_OK; tn = tn == 16 ? 32 : tn * 4) {
           const int64_t units = rb_n * (m > tn ? (m + tn - 1) / tn : 1);
           int splits = 1;
-          rc = choose_splits(kind, tn, units, k_stages, dev, &splits);
+          rc = fp8_splits(tn, units, k_stages, dev, &splits);
           const float t = fp8_few_time(tn, m, units, k_stages, splits, dev.sm_count);
           if (tn == 16 || t < least) {
             least = t;

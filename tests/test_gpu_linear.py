@@ -199,6 +199,23 @@ def test_many_tiles_strided_output(cuda_device, kind, dtype, pad, shift):
     assert torch.equal(full.cpu(), want)
 
 
+# Token tiles of the 4-bit kernels for few rows with K split over clusters, and of 128 tokens on shared SMs.
+@pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m,n,k,tile", [(9, 300, 8192, 16), (30, 129, 8192, 32), (51, 300, 8192, 64), (64, 1000, 14336, 64),
+                                        (100, 300, 8192, 128), (257, 700, 12320, 128), (190, 9217, 8192, 128)])
+def test_exact_fp4_splits(cuda_device, kind, m, n, k, tile):
+    gen = torch.Generator().manual_seed(m)
+    x, w = _exact_operand(kind, m, k, gen, False), _exact_operand(kind, n, k, gen, True)
+    want = (_decode(x).to(cuda_device) @ _decode(w).to(cuda_device).T).float()
+    d = torch.full((m + 2, n + 3), 7.0, device=cuda_device)
+    plan = lowp.LowpLinearPlan(x.to(cuda_device), w.to(cuda_device), d[:m, :n])
+    assert plan.info["few_rows"] and plan.info["tile_m"] == tile and plan.info["k_splits"] > 1
+    plan.run(3)
+    plan.synchronize()
+    assert torch.equal(d[:m, :n], want)
+    assert (d[m:] == 7).all() and (d[:, n:] == 7).all()
+
+
 # Three waves of 256 x 256 tiles and a long K: CTA pairs for every kind; a few K: one CTA per tile.
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("m,n,k,pad,dtype,pairs", [
