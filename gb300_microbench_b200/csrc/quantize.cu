@@ -2,7 +2,7 @@
 //
 //   RMS norm with the residual's addition and FP8 output (bb_rmsnorm_fp8_*)
 //     h = round_T(x + r),  y = h * rsqrt(mean(h^2) + eps) * w,
-//     s[g] = amax |y[g]| / 448 over the 128 columns of group g (1 where that is 0),
+//     s[g] = amax |y[g]| / 448 over the 128 columns of group g (1 where that is 0 in FP32),
 //     q = e4m3(y / s), the scales stored [group][row].
 //   4-bit microscaled formats (bb_fp4_quant_*)
 //     NVFP4: b = e4m3(min(amax_16 / 6 / g, 448)), q = e2m1(x / (b g)), 0 where b g is 0
@@ -293,7 +293,10 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_fp8_kernel(const NormPara
       for (int d = kLanes / 2; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
       const int cg = kWide ? c : c - lane + 128 * g;  // wide: anywhere in the group; else its first column
       if (cg >= p.cols) continue;
-      const float s = amax == 0.f ? 1.f : __fdiv_rn(amax, kE4m3Max);
+      // 1 where the quotient is 0, which a group below 448 times the least FP32
+      // number rounds to as well; a NaN stays.
+      const float quotient = __fdiv_rn(amax, kE4m3Max);
+      const float s = quotient == 0.f ? 1.f : quotient;
       if (lane % kLanes == 0) p.scales[(cg / 128) * p.s_ld + row] = s;
       // Rounded quotients here too: a product with the rounded reciprocal moves
       // two to four times as many values across a border of the E4M3 grid as

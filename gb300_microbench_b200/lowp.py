@@ -181,13 +181,14 @@ def fp8_block_dequantize(q: torch.Tensor, scale: torch.Tensor, block: int = 128)
 
 def fp8_group_quantize(x: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
     """x (R, K) -> (E4M3 bits (R, K) uint8, FP32 scales (R, ceil(K/128)))
-    with scale = amax(group) / 448, 1 where that is 0."""
+    with scale = amax(group) / 448, 1 where that is 0 in FP32."""
     x = x.float()
     r, k = x.shape
     kb = -(-k // group)
     blocks = torch.nn.functional.pad(x, (0, kb * group - k)).view(r, kb, group)
     amax = blocks.abs().amax(dim=2)
-    scale = torch.where(amax == 0, torch.ones_like(amax), amax / torch.full_like(amax, E4M3_MAX))
+    scale = amax / torch.full_like(amax, E4M3_MAX)
+    scale = torch.where(scale == 0, torch.ones_like(scale), scale)
     q = (blocks / scale[:, :, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
     return q.view(r, kb * group)[:, :k].contiguous().view(torch.uint8), scale
 

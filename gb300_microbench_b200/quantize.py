@@ -79,7 +79,7 @@ class RmsNormFp8Plan(_QuantPlan):
 
         h = x + residual                   (rounded to x's dtype; h = x without a residual)
         y = h * rsqrt(mean(h^2) + eps) * weight
-        s = max|y| / 448                   per row and 128 columns, 1 where that is 0
+        s = max|y| / 448                   per row and 128 columns, 1 where that is 0 in FP32
         out = e4m3(y / s), out.scales = s
 
     ``x``, ``residual`` and ``residual_out`` are (rows, cols) bfloat16, float16

@@ -350,7 +350,7 @@ BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, cons
 /* h = x + residual rounded to x's dtype (residual NULL: h = x), stored to
  * residual_out where that is not NULL (it may be residual or x); y = h *
  * rsqrt(mean(h^2) + eps) * weight; q = E4M3 of y / s (row stride q_ld) with s =
- * max|y| / 448 over each 128 columns (1 where that is 0), stored to
+ * max|y| / 448 over each 128 columns (1 where that is 0 in FP32), stored to
  * scales[group * scales_ld + row]. cols up to 65536; weight is FP32 or of x's
  * dtype. A row that holds a NaN or an infinity is NaN. */
 BB_API int bb_rmsnorm_fp8_plan_create(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t x_ld,

@@ -105,6 +105,31 @@ def test_norm_zero_and_non_finite_rows(cuda_device):
     assert torch.isnan(q[3, 5]) and torch.isnan(s[3, 0])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [640, 637])
+def test_norm_groups_below_the_scales_range(cuda_device, dtype, cols):
+    """Groups whose max|y| / 448 is 0 in FP32 beside ordinary ones: scale 1, codes 0. Weights below 2^-10 take BF16's
+    least numbers there too. A group a little above has a subnormal scale and finite codes."""
+    x = torch.zeros(4, cols, dtype=dtype)
+    x[:, 512:] = _x(4, cols - 512, dtype, seed=6)
+    w = torch.ones(cols)
+    w[:512] = 2.0 ** -13
+    _, q0, s0 = _norm(x, w, cuda_device, store=False)
+    _norm_check(x, None, w, 1e-6, None, q0, s0)
+    x[:, 3] = 2.0 ** -133  # y is about 2^-145, less than 448 * 2^-150
+    x[1:, 129] = -2.0 ** -133
+    x[2, 260], x[3, 300] = 2.0 ** -125, 2.0 ** -133
+    _, q, s = _norm(x, w, cuda_device, store=False)
+    assert torch.equal(q[:, 512:], q0[:, 512:]) and torch.equal(s[:, 4], s0[:, 4])  # their squares are 0
+    assert torch.isfinite(q).all() and torch.isfinite(s).all()
+    low = torch.ones(4, 512, dtype=torch.bool)
+    low[2, 256:384] = False
+    assert not q[:, :512][low].any()
+    assert torch.equal(s[:, :2], torch.ones(4, 2)) and torch.equal(s[:, 3], torch.ones(4))
+    assert s[2, 2] > 0 and s[2, 2] < 2.0 ** -126 and torch.equal(s[[0, 1, 3], 2], torch.ones(3))
+    assert (q[2, 256:384] != 0).nonzero().flatten().tolist() == [4]
+
+
 def test_norm_no_rows(cuda_device):
     x = torch.empty(0, 64, dtype=torch.bfloat16)
     h, q, s = _norm(x, torch.ones(64), cuda_device)

@@ -86,6 +86,23 @@ def test_fp8_group_format():
     assert ((got - x.double()).abs() <= bound).all()
 
 
+def test_fp8_groups_below_the_scales_range():
+    """amax / 448 below half the least FP32 number (1.4e-45) is 0: such a group has scale 1 and codes 0. From there
+    on the scale is a subnormal number and no code is NaN."""
+    x = torch.zeros(3, 384)
+    x[0, 0], x[0, 130], x[0, 300] = 1e-43, -3e-43, 2.0 ** -149
+    x[1, 7], x[1, 129], x[1, 257] = 1e-42, -5e-41, 1.0
+    q, s = lowp.fp8_group_quantize(x)
+    v = q.view(torch.float8_e4m3fn).float()
+    assert torch.equal(s[0], torch.ones(3)) and torch.equal(s[2], torch.ones(3))
+    assert not v[0].any() and not v[2].any()
+    assert (s[1] > 0).all() and torch.isfinite(v).all()
+    assert (v[1] != 0).nonzero().flatten().tolist() == [7, 129, 257]
+    # The scale is off by half of 2^-149 at most, or 448 times that once multiplied back; the code by half a step.
+    got = lowp.fp8_group_dequantize(q, s).double()
+    assert ((got - x.double()).abs() <= x.double().abs() * 2.0 ** -4 + 448 * 2.0 ** -150 + 2.0 ** -150).all()
+
+
 @pytest.mark.parametrize("rows,width", [(1, 1), (130, 5), (128, 8), (257, 90)])
 def test_scale_atoms_round_trip(rows, width):
     s = torch.randint(0, 256, (rows, width), dtype=torch.uint8, generator=torch.Generator().manual_seed(rows))
