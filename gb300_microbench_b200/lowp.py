@@ -160,7 +160,7 @@ def _extents(rows: int, k: int, step: int) -> tuple[int, int]:
 
 def fp8_block_quantize(x: torch.Tensor, block: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
     """x (R, K) -> (E4M3 bits (R, K) uint8, FP32 scales (ceil(R/128), ceil(K/128)))
-    with scale = amax(block) / 448."""
+    with scale = amax(block) / 448, 1 where that is 0 in FP32 or NaN."""
     x = x.float()
     r, k = x.shape
     rb, kb = -(-r // block), -(-k // block)
@@ -168,7 +168,8 @@ def fp8_block_quantize(x: torch.Tensor, block: int = 128) -> tuple[torch.Tensor,
     pad[:r, :k] = x
     blocks = pad.view(rb, block, kb, block)
     amax = blocks.abs().amax(dim=(1, 3))
-    scale = torch.where(amax > 0, amax / E4M3_MAX, torch.ones_like(amax))
+    scale = amax / E4M3_MAX
+    scale = torch.where(scale > 0, scale, torch.ones_like(scale))
     q = (blocks / scale[:, None, :, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
     return q.view(rb * block, kb * block)[:r, :k].contiguous().view(torch.uint8), scale.contiguous()
 

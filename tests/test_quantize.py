@@ -103,6 +103,20 @@ def test_fp8_groups_below_the_scales_range():
     assert ((got - x.double()).abs() <= x.double().abs() * 2.0 ** -4 + 448 * 2.0 ** -150 + 2.0 ** -150).all()
 
 
+def test_fp8_blocks_below_the_scales_range():
+    """The weights' 128 x 128 blocks likewise: scale 1 and codes 0 where amax / 448 is 0 in FP32."""
+    x = torch.zeros(200, 256)
+    x[5, 3], x[9, 4] = 1e-43, -3e-43
+    x[130, 7], x[131, 200] = 1e-42, 2.0
+    q, s = lowp.fp8_block_quantize(x)
+    v = q.view(torch.float8_e4m3fn).float()
+    assert torch.isfinite(v).all() and (s > 0).all()
+    assert torch.equal(s[0], torch.ones(2)) and not v[:128].any()
+    assert (v != 0).nonzero().tolist() == [[130, 7], [131, 200]]
+    got = lowp.fp8_block_dequantize(q, s).double()
+    assert ((got - x.double()).abs() <= x.double().abs() * 2.0 ** -4 + 448 * 2.0 ** -150 + 2.0 ** -150).all()
+
+
 @pytest.mark.parametrize("rows,width", [(1, 1), (130, 5), (128, 8), (257, 90)])
 def test_scale_atoms_round_trip(rows, width):
     s = torch.randint(0, 256, (rows, width), dtype=torch.uint8, generator=torch.Generator().manual_seed(rows))
