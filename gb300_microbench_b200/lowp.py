@@ -385,6 +385,20 @@ def config4_inputs(m: int, n: int, k: int, seed: int = 0, device: str | torch.de
 KINDS = {"nvfp4": nat.BB_LOWP_NVFP4, "fp8_block128": nat.BB_LOWP_FP8_BLOCK128}
 
 
+_GEMM_OPERANDS = {"nvfp4": Nvfp4Operand, "fp8_block128": Fp8BlockOperand, "fp8_tensor_scaled": Fp8BlockOperand}
+
+
+def _check_operands(kind: str, a, b) -> None:
+    """Operands of the kind's own class: the classes share attribute names
+    whose layouts differ (an Fp8GroupOperand's scales are per row)."""
+    want = _GEMM_OPERANDS[kind]
+    for name, op in (("A", a), ("B", b)):
+        if not isinstance(op, want):
+            raise ValueError(f"{name} is {type(op).__name__}, {kind} takes {want.__name__}")
+        if kind == "nvfp4" and op.tensor_scale is None:
+            raise ValueError(f"{name}'s tensor scale is found on the GPU, where only LowpLinearPlan reads it")
+
+
 def _check_buffers(kind: str, a, b, d: torch.Tensor, sfa: torch.Tensor, sfb: torch.Tensor, stream) -> None:
     """Every buffer on D's device, contiguous, and at least as large as the
     native side reads: its tensor maps and scale loads are sized from M, N
@@ -412,11 +426,14 @@ def _check_buffers(kind: str, a, b, d: torch.Tensor, sfa: torch.Tensor, sfb: tor
 
 class LowpGemmPlan:
     """D (M, N) BF16 = dequant(A) @ dequant(B)^T through the sm_100a
-    block-scaled kernel (bb_lowp_plan_create of include/b200bench.h)."""
+    block-scaled kernel (bb_lowp_plan_create of include/b200bench.h). A and B
+    are :class:`Nvfp4Operand` for "nvfp4" (with a tensor scale known on the
+    host) and :class:`Fp8BlockOperand` for "fp8_block128"."""
 
     def __init__(self, kind: str, a, b, d: torch.Tensor, stream: torch.cuda.Stream | None = None):
         if kind not in KINDS:
             raise ValueError(f"unknown kind {kind!r}; expected one of {sorted(KINDS)}")
+        _check_operands(kind, a, b)
         if not d.is_cuda or d.dtype != torch.bfloat16 or not d.is_contiguous():
             raise ValueError("D must be a contiguous CUDA bfloat16 tensor")
         self.kind = kind
@@ -484,6 +501,7 @@ class CublasLtLowpPlan:
         FP8 block-scaled kernel, not the same function."""
         if kind not in self.CMP_KINDS:
             raise ValueError(f"unknown kind {kind!r}")
+        _check_operands(kind, a, b)
         self._lib = nat.cmp_lib()
         self.stream = stream if stream is not None else torch.cuda.current_stream(d.device)
         m, n, k = a.rows, b.rows, a.k

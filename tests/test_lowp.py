@@ -110,3 +110,21 @@ def test_scale_bytes_contract():
     assert lib.bb_lowp_scale_bytes(nat.BB_LOWP_FP8_BLOCK128, 300, 384) == 3 * 3 * 4
     assert lib.bb_lowp_scale_bytes(nat.BB_LOWP_NVFP4, 300, 100) == -1
     assert lib.bb_lowp_scale_bytes(9, 300, 384) == -1
+
+
+def test_plans_refuse_operands_of_another_class():
+    """At K = 128 an Fp8GroupOperand's scales (R, 1) would pass for those of 128 x 128 blocks."""
+    d = torch.zeros(128, 128, dtype=torch.bfloat16)
+    x = torch.ones(128, 128)
+    group, block, nv, mx = (c(x) for c in (lowp.Fp8GroupOperand, lowp.Fp8BlockOperand, lowp.Nvfp4Operand, lowp.Mxfp4Operand))
+    found = lowp.Nvfp4Operand.empty(128, 128, device="cpu")
+    for plan in (lowp.LowpGemmPlan, lowp.CublasLtLowpPlan):
+        for kind, a, b, match in (("fp8_block128", group, block, "A is Fp8GroupOperand"),
+                                  ("fp8_block128", block, group, "B is Fp8GroupOperand"),
+                                  ("fp8_block128", nv, nv, "A is Nvfp4Operand"), ("nvfp4", block, block, "A is Fp8BlockOperand"),
+                                  ("nvfp4", mx, nv, "A is Mxfp4Operand"), ("nvfp4", nv, mx, "B is Mxfp4Operand"),
+                                  ("nvfp4", found, nv, "tensor scale"), ("nvfp4", nv, found, "tensor scale")):
+            with pytest.raises(ValueError, match=match):
+                plan(kind, a, b, d)
+    with pytest.raises(ValueError, match="CUDA"):
+        lowp.LowpGemmPlan("fp8_block128", block, block, d)
