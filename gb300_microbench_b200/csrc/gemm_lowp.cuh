@@ -736,11 +736,20 @@ __global__ void __launch_bounds__(Cfg<kKind, kCG>::THREADS, 1)
         constexpr bool kGroup = kKind == kFp8Group;
         constexpr int kAhead = 4;
         const float* sa_lane = sa + min(row, p.m - 1);
+        // A linear layer's launch may begin while the kernel in front still
+        // writes the scales; the non-coherent path is for memory that nobody
+        // writes as long as the kernel lives.
+        auto load_scale = [](const float* at) {
+          if constexpr (!kLinear) return __ldg(at);
+          float v;
+          asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(at));
+          return v;
+        };
         float sa_next[kAhead];
         if constexpr (kGroup) {
 #pragma unroll
           for (int j = 0; j < kAhead; ++j) {
-            sa_next[j] = j < p.k_stages ? __ldg(sa_lane) : 0.f;
+            sa_next[j] = j < p.k_stages ? load_scale(sa_lane) : 0.f;
             sa_lane += p.sfa_ld;
           }
         }
@@ -759,8 +768,8 @@ __global__ void __launch_bounds__(Cfg<kKind, kCG>::THREADS, 1)
           ra = 0.f;
           rb = 0.f;
           if (kk < p.k_stages) {
-            ra = kGroup ? 1.f : __ldg(sa_row + kk);
-            rb = __ldg(sb_row + kk);
+            ra = kGroup ? 1.f : load_scale(sa_row + kk);
+            rb = load_scale(sb_row + kk);
           }
         };
         load_raw(lane);
@@ -776,7 +785,7 @@ __global__ void __launch_bounds__(Cfg<kKind, kCG>::THREADS, 1)
             s *= sa_next[0];
 #pragma unroll
             for (int j = 0; j + 1 < kAhead; ++j) sa_next[j] = sa_next[j + 1];
-            if (ks + kAhead < p.k_stages) sa_next[kAhead - 1] = __ldg(sa_lane);
+            if (ks + kAhead < p.k_stages) sa_next[kAhead - 1] = load_scale(sa_lane);
             sa_lane += p.sfa_ld;
           }
           const uint32_t buf = acc_iter % C::FP8_BUFS;

@@ -301,6 +301,60 @@ def test_weights_quantised_just_before(cuda_device, fmt):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n,k,pairs", [(2300, 4304, 8192, True), (1400, 3304, 576, False)])
+def test_activations_quantised_just_before(cuda_device, kind, m, n, k, pairs):
+    """Quantiser and tile kernel in turn with nothing between them, each launch starting before the one in
+    front has ended: every product is of its own step's tokens and scales, which lie at one address."""
+    gen = torch.Generator(device=cuda_device).manual_seed(9)
+    w = {"fp8": lowp.Fp8BlockOperand, "mxfp4": lowp.Mxfp4Operand, "nvfp4": lowp.Nvfp4Operand}[kind](
+        torch.randn(n, k, generator=gen, device=cuda_device))
+    empty = {"fp8": lowp.Fp8GroupOperand, "mxfp4": lowp.Mxfp4Operand, "nvfp4": lowp.Nvfp4Operand}[kind].empty
+    weight = torch.ones(k, device=cuda_device)
+
+    def quantiser(x, a, i):
+        return quantize.RmsNormFp8Plan(x, weight * 4.0 ** i, a) if kind == "fp8" else quantize.Fp4QuantPlan(x, a)
+
+    shared = empty(m, k, device=cuda_device)
+    steps, want = [], []
+    for i in range(5):
+        x = torch.randn(m, k, generator=gen, device=cuda_device) * 4.0 ** (i - 2)
+        x *= torch.exp(torch.randn(m, 1, generator=gen, device=cuda_device))
+        x = x.to(torch.bfloat16)
+        alone = empty(m, k, device=cuda_device)
+        plans = [quantiser(x, alone, i)] + [lowp.LowpLinearPlan(alone, w, torch.empty(m, n, dtype=torch.bfloat16, device=cuda_device))]
+        for p in plans:
+            p.run()
+            p.synchronize()
+        want.append(plans[1].d)
+        rows = torch.randint(0, m, (16,), generator=gen, device=cuda_device)
+        _check(_rows_of(alone.to("cpu"), rows.cpu()), w.to("cpu"), plans[1].d[rows].cpu())
+        product = lowp.LowpLinearPlan(shared, w, torch.empty(m, n, dtype=torch.bfloat16, device=cuda_device))
+        assert product.info["few_rows"] == 0 and product.info["cta_group"] == (2 if pairs else 1)
+        steps.append((quantiser(x, shared, i), product))
+    torch.cuda.synchronize(cuda_device)
+    for _ in range(4):
+        for _, product in steps:
+            product.d.zero_()
+        for quantiser_, product in steps:
+            quantiser_.run()
+            product.run()
+        torch.cuda.synchronize(cuda_device)
+        for (_, product), d in zip(steps, want):
+            product.synchronize()
+            assert torch.equal(product.d, d)
+
+
+def _rows_of(op, rows):
+    """The operand of some of its rows."""
+    if isinstance(op, lowp.Fp8GroupOperand):
+        return lowp.Fp8GroupOperand.from_parts(op.data[rows], op.scales[rows])
+    mx = isinstance(op, lowp.Mxfp4Operand)
+    bits = lowp.unpack_scale_atoms(op.atoms, op.rows, op.k // (32 if mx else 16))[rows]
+    return lowp.Mxfp4Operand.from_parts(op.data[rows], bits) if mx else \
+        lowp.Nvfp4Operand.from_parts(op.data[rows], bits, float(op.tensor_scale_out))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_nan_stays_in_its_row(cuda_device, kind):
     gen = torch.Generator().manual_seed(5)
     k, n = 256, 136
