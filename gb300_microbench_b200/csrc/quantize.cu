@@ -158,7 +158,10 @@ __device__ __forceinline__ F2 pair_f32(const Vec<T>& v, int i) {
 }
 
 // One CTA per row; a thread's kIters vectors of 32 bytes stay in registers
-// between the sum and the output, so x and r are read once. 16384 x 8192 BF16:
+// between the sum and the output, so x and r are read once. (Rows that take 1024
+// threads have 64 registers each: 16-bit rows above 32768 columns keep up to 24
+// words a thread in local memory, FP32 rows above 16384 112 to 134. One CTA per
+// SM there: FP32 1024 x 32768 176 us; with 32 registers, for two, 273.) 16384 x 8192 BF16:
 // 138 us, 6.8 TB/s of the 940 MB it moves; what it took were 256-bit accesses,
 // packed FP32 and 16-bit arithmetic (at twice the instructions the issue slots
 // were 76 % busy and it took 168 us) and all loads in flight before the first store.
@@ -169,7 +172,7 @@ __device__ __forceinline__ F2 pair_f32(const Vec<T>& v, int i) {
 // access is a coalesced one of single elements, and 4 elements of each lane
 // make a group.
 template <typename T, int kIters, bool kWide, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads) rmsnorm_fp8_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 1024 ? 1 : 0) rmsnorm_fp8_kernel(const NormParams p) {
   constexpr int VE = kVE<T>;
   __shared__ float warp_sum[32];
   grid_wait();
@@ -233,17 +236,51 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_fp8_kernel(const NormPara
       }
     }
   }
-  float sum, odd;
-  unpack2(sum2, sum, odd);
-  sum += odd;
+  // The CTA's sum, the same in every thread.
+  auto block_sum = [&](F2 of_thread) {
+    float sum, odd;
+    unpack2(of_thread, sum, odd);
+    sum += odd;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane == 0) warp_sum[threadIdx.x / 32] = sum;
-  __syncthreads();
-  sum = lane < blockDim.x / 32 ? warp_sum[lane] : 0.f;
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) warp_sum[threadIdx.x / 32] = sum;
+    __syncthreads();
+    sum = lane < blockDim.x / 32 ? warp_sum[lane] : 0.f;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  const float rstd = rsqrtf(sum / static_cast<float>(p.cols) + p.eps);
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum;
+  };
+  float var = block_sum(sum2) / static_cast<float>(p.cols) + p.eps;
+  float rstd = rsqrtf(var);
+  // Squares that leave FP32's range, or sink below 2^-100 where eps does not
+  // cover them, are taken again of h times a power of two. FP16's stay inside.
+  // Small rows keep the factor, since 1 / rms may be no FP32 number. (NaN and
+  // infinite rows come here too and stay what they are.)
+  if (!std::is_same_v<T, __half> && !(var >= 0x1p-100f && var < __int_as_float(0x7f800000))) {
+    const bool small = var < 1.f;
+    const float f = small ? 0x1p100f : 0x1p-80f;
+    const F2 f2 = pack2(f, f);
+    sum2 = pack2(0.f, 0.f);
+#pragma unroll
+    for (int it = 0; it < kIters; ++it) {
+      if (first(it) < p.cols) {
+#pragma unroll
+        for (int i = 0; i < VE / 2; ++i) {
+          const F2 h = mul2(pair_f32(v[it], i), f2);
+          sum2 = fma2(h, h, sum2);
+          if (small) {
+            float lo, hi;
+            unpack2(h, lo, hi);
+            v[it].e[2 * i] = from_f32<T>(lo);  // exact
+            v[it].e[2 * i + 1] = from_f32<T>(hi);
+          }
+        }
+      }
+    }
+    __syncthreads();  // the first sum has been read
+    var = block_sum(sum2) / static_cast<float>(p.cols) + p.eps * f * f;
+    rstd = small ? rsqrtf(var) : rsqrtf(var) * f;
+  }
   const F2 rstd2 = pack2(rstd, rstd);
 #pragma unroll
   for (int it = 0; it < kIters; ++it) {

@@ -86,7 +86,11 @@ class RmsNormFp8Plan(_QuantPlan):
     or float32 of one dtype, with unit column stride; ``residual_out`` receives
     h (it may be ``residual`` or ``x``; by default the sum is not stored).
     ``weight`` is (cols,), of x's dtype or float32. cols is at most 65536;
-    rows may be 0. A row that holds a NaN or an infinity comes out as NaN."""
+    rows may be 0. Finite rows are right up to the ends of x's range, where
+    squares leave FP32's. A row that holds a NaN is NaN, scales and codes. In one
+    that holds an infinity the formula gives NaN for its 128 columns and, as
+    1 / rms is 0, codes 0 with scale 1 for the others: a product's row of either
+    is NaN. With eps = 0 a row of zeros is NaN (0 / 0)."""
 
     def __init__(self, x: torch.Tensor, weight: torch.Tensor, out: Fp8GroupOperand, residual: torch.Tensor | None = None,
                  residual_out: torch.Tensor | None = None, eps: float = 1e-6,

@@ -105,6 +105,56 @@ def test_norm_zero_and_non_finite_rows(cuda_device):
     assert torch.isnan(q[3, 5]) and torch.isnan(s[3, 0])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [640, 637])
+def test_norm_infinite_rows(cuda_device, dtype, cols):
+    """The whole row: NaN in the infinity's group of 128, 0 with scale 1 in the others; by the residual's
+    addition too."""
+    big = torch.finfo(dtype).max
+    x, res = _x(4, cols, dtype, seed=7), torch.zeros(4, cols, dtype=dtype)
+    x[1, 200], x[2, cols - 1] = float("inf"), -float("inf")
+    x[3, 5] = res[3, 5] = big
+    w = torch.ones(cols)
+    h, q, s = _norm(x, w, cuda_device, res)
+    _norm_check(x[:1], res[:1], w, 1e-6, h[:1], q[:1], s[:1])
+    assert torch.isinf(h[3, 5])
+    for r, group in ((1, 1), (2, 4), (3, 0)):
+        inside = torch.zeros(cols, dtype=torch.bool)
+        at = {1: 200, 2: cols - 1, 3: 5}[r]
+        inside[128 * group:128 * (group + 1)] = True
+        # The group's scale is NaN, and so are all its codes.
+        assert torch.isnan(q[r, at]) and torch.isnan(q[r, inside]).all() and torch.isnan(s[r, group])
+        assert not q[r, ~inside].any()
+        assert torch.equal(s[r, torch.arange(5) != group], torch.ones(4))
+
+
+# Rows whose squares leave FP32, upwards and (with eps 0, which does not cover them) downwards.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [300, 4096, 12288, 32776, 65536])
+@pytest.mark.parametrize("magnitude,eps", [(3e38, 1e-6), (1e30, 0.0), (1e19, 1e-6), (1e18, 1e-6), (1e-14, 0.0), (1e-16, 0.0),
+                                           (1e-16, 1e-32), (1e-22, 1e-33), (1e-30, 0.0), (1e-37, 0.0)])
+def test_norm_squares_outside_fp32(cuda_device, dtype, cols, magnitude, eps):
+    x = _x(3, cols, torch.float32, seed=8)
+    x = (x / x.abs().max() * magnitude).to(dtype)
+    x[1, cols // 2:] = 0
+    x[1, -1] = magnitude / 1024
+    x[2] = _x(1, cols, dtype, seed=9)[0]  # an ordinary row beside them
+    w = torch.linspace(0.5, 2, cols)
+    assert torch.isfinite(x).all()
+    h, q, s = _norm(x, w, cuda_device, store=True, eps=eps)
+    _norm_check(x, None, w, eps, h, q, s)
+
+
+def test_norm_least_numbers(cuda_device):
+    """Rows of the types' least numbers: 1 / rms lies outside FP32, the result does not."""
+    for dtype, least in ((torch.bfloat16, 2.0 ** -133), (torch.float32, 2.0 ** -149), (torch.float16, 2.0 ** -24)):
+        x = torch.full((2, 384), least, dtype=dtype)
+        x[1, 1::2] = 0
+        _, q, s = _norm(x, torch.ones(384), cuda_device, store=False, eps=0.0)
+        _norm_check(x, None, torch.ones(384), 0.0, None, q, s)
+        assert (q[0] == 448).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("cols", [640, 637])
 def test_norm_groups_below_the_scales_range(cuda_device, dtype, cols):
