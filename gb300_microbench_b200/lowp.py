@@ -337,12 +337,19 @@ class Fp8GroupOperand:
         return op
 
     @property
+    def data(self) -> torch.Tensor:
+        return self._data
+
+    @data.setter
+    def data(self, data: torch.Tensor) -> None:
+        self._data, self._values = data, None
+
+    @property
     def values(self) -> torch.Tensor:
         """The E4M3 values, (R, K) float8_e4m3fn (a view of ``data``)."""
-        view = self.__dict__.get("_values")
-        if view is None or view.data_ptr() != self.data.data_ptr():
-            view = self._values = self.data.view(torch.float8_e4m3fn)
-        return view
+        if self._values is None:  # one view per assigned ``data``: making one takes a microsecond
+            self._values = self._data.view(torch.float8_e4m3fn)
+        return self._values
 
     def to(self, device) -> "Fp8GroupOperand":
         return Fp8GroupOperand.from_parts(self.data.to(device), self.scales.to(device))

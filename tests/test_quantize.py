@@ -143,6 +143,23 @@ def test_operands_refuse_what_does_not_fit():
     assert op.scales.shape == (5, 3) and op.scales.stride() == (1, 5) and op.values.dtype == torch.float8_e4m3fn
 
 
+def test_values_follow_the_data():
+    """``values`` is of the tensor that is ``data`` now, also where a new one begins at the old one's address."""
+    op = lowp.Fp8GroupOperand.empty(5, 130, device="cpu")
+    op.data.fill_(0x38)
+    assert op.values.shape == (5, 130) and (op.values.float() == 1).all()
+    first = op.data
+    first.fill_(0x40)
+    assert (op.values.float() == 2).all()
+    op.data = first[:2]
+    assert op.values.shape == (2, 130) and op.values.data_ptr() == first.data_ptr()
+    op.data = torch.full((3, 130), 0x38, dtype=torch.uint8)
+    assert op.values.shape == (3, 130) and (op.values.float() == 1).all()
+    op.data = op.data.view(torch.float8_e4m3fn)
+    assert op.values.shape == (3, 130) and (op.values.float() == 1).all()
+    assert torch.equal(op.to("cpu").values.view(torch.uint8), op.data.view(torch.uint8))
+
+
 def test_plans_refuse_before_any_launch():
     """Shapes, dtypes and strides are refused in Python, CPU tensors among them."""
     x = torch.zeros(4, 64, dtype=torch.bfloat16)
