@@ -157,6 +157,7 @@ def test_values_follow_the_data():
     assert op.values.shape == (3, 130) and (op.values.float() == 1).all()
     op.data = op.data.view(torch.float8_e4m3fn)
     assert op.values.shape == (3, 130) and (op.values.float() == 1).all()
+    op.rows, op.scales = 3, torch.ones(2, 3).t()
     assert torch.equal(op.to("cpu").values.view(torch.uint8), op.data.view(torch.uint8))
 
 
