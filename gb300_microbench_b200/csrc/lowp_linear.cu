@@ -210,6 +210,11 @@ __global__ void __launch_bounds__(FewCfg<kKind, kTN>::THREADS, FewCfg<kKind, kTN
                     const FewParams p) {
   using C = FewCfg<kKind, kTN>;
   constexpr int STAGES = C::STAGES;
+  if (blockDim.x != C::THREADS || p.splits < 1 || cluster_nctarank() != static_cast<uint32_t>(p.splits) ||
+      gridDim.x % p.splits != 0) {
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kDevBadLaunch);
+    return;
+  }
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_w = smem;
