@@ -546,3 +546,29 @@ def test_captured_fork_and_join(cuda_device, kind):
         _check(a.to("cpu"), w.to("cpu"), behind.cpu())
         if kind == "mxfp4":
             assert torch.equal(a.data.cpu(), lowp.mxfp4_quantize(src.cpu())[0])
+
+
+@pytest.mark.parametrize("op", ["norm_fp8", "fp4_quantize", "fp4_linear"])
+def test_measured_pass_under_another_stream(cuda_device, op, monkeypatch):
+    """A pass of perf/operators.py under a stream that is not its plans': behind the copy that fills x there,
+    and before what reads the outputs there."""
+    from perf import operators
+
+    monkeypatch.setattr(operators, "own", True)
+    case = next(c for c in operators.listed() if c["op"] == op)
+    s, other = operators.prepare(case, 1), operators.prepare(case, 2)
+    first = {k: v.clone() for k, v in operators.run(s).items()}
+    x = s["x"].clone()
+    s["x"].copy_(other["x"])
+    operators.run(s)  # what stale outputs would hold
+    torch.cuda.synchronize(cuda_device)
+    side = torch.cuda.Stream(device=cuda_device)
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            torch.cuda._sleep(20_000_000)  # about 10 ms
+            s["x"].copy_(x)
+            got = {k: v.clone() for k, v in operators.run(s).items()}
+            s["x"].copy_(other["x"])
+    torch.cuda.synchronize(cuda_device)
+    for k, v in first.items():
+        assert torch.equal(got[k].contiguous().view(torch.uint8), v.contiguous().view(torch.uint8))
