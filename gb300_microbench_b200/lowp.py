@@ -592,6 +592,11 @@ class LowpLinearPlan:
         fp8 = self.kind == "fp8_group128"
         sx, sw = (x.scales, w.scales) if fp8 else (x.atoms, w.atoms)
         scale_devs = [None if fp8 else getattr(op, "tensor_scale_out", None) for op in (x, w)]
+        for name, t in (("x data", x.data), ("w data", w.data)) + (() if fp8 else (("x atoms", sx), ("w atoms", sw))):
+            if t.element_size() != 1:
+                raise ValueError(f"{name} is {t.dtype}, expected one byte an element")
+        if fp8 and sw.dtype != torch.float32:
+            raise ValueError(f"w scales are {sw.dtype}, expected torch.float32")
         tensors = [x.data, w.data, sx, sw, d] + [t for t in scale_devs if t is not None]
         if not all(t.is_cuda for t in tensors):
             raise ValueError("operands and D must be CUDA tensors")

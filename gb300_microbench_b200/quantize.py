@@ -107,8 +107,8 @@ class RmsNormFp8Plan(_QuantPlan):
             raise ValueError(f"weight is {weight.dtype}, expected {x.dtype} or torch.float32")
         if not eps >= 0:
             raise ValueError("eps must not be negative")
-        if not out.data.is_contiguous() or out.data.numel() < out.rows * out.k:
-            raise ValueError("out.data must be contiguous (rows, cols)")
+        if not out.data.is_contiguous() or out.data.numel() < out.rows * out.k or out.data.element_size() != 1:
+            raise ValueError("out.data must be contiguous (rows, cols) of one byte an element")
         s = out.scales
         if tuple(s.shape) != (out.rows, -(-out.k // 128)) or (out.rows > 1 and s.stride(0) != 1) or (
                 s.shape[1] > 1 and s.stride(1) < out.rows) or s.dtype != torch.float32:
@@ -160,8 +160,8 @@ class Fp4QuantPlan(_QuantPlan):
         per_atom = 64 if nvfp4 else 128
         atoms = -(-out.rows // 128) * -(-out.k // per_atom) * 512
         if not out.data.is_contiguous() or out.data.numel() < out.rows * out.k // 2 or not out.atoms.is_contiguous() \
-                or out.atoms.numel() < atoms:
-            raise ValueError("out.data and out.atoms must be contiguous and hold (rows, K/2) and all atoms")
+                or out.atoms.numel() < atoms or out.data.element_size() != 1 or out.atoms.element_size() != 1:
+            raise ValueError("out.data and out.atoms must be contiguous bytes and hold (rows, K/2) and all atoms")
         tensors = [t for t in (x, values, out.data, out.atoms, scale_out) if t is not None]
         self.stream = _one_device(tensors, stream)
         self.x, self.out, self.values, self._keep = x, out, values, tensors

@@ -204,6 +204,30 @@ def test_plans_refuse_before_any_launch():
             pytest.fail(f"case {i} was accepted")
 
 
+def test_plans_refuse_buffers_of_other_types():
+    """Large enough in bytes, but not the bytes that the kernels read."""
+    x, d = torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(4, 256, dtype=torch.bfloat16)
+    a8, b8 = lowp.Fp8GroupOperand.empty(4, 128, device="cpu"), lowp.Fp8BlockOperand(torch.ones(256, 128))
+    a4, b4 = lowp.Mxfp4Operand.empty(4, 128, device="cpu"), lowp.Mxfp4Operand(torch.ones(256, 128))
+    floats = lowp.Fp8BlockOperand.from_parts(torch.ones(256, 128), torch.ones(2, 1))
+    doubles = lowp.Fp8BlockOperand(torch.ones(256, 128))
+    doubles.scales = doubles.scales.double()
+    words = lowp.Mxfp4Operand(torch.ones(256, 128))
+    words.atoms = words.atoms.int()
+    wide8, wide4 = lowp.Fp8GroupOperand.empty(4, 128, device="cpu"), lowp.Mxfp4Operand.empty(4, 128, device="cpu")
+    wide8.data, wide4.data = wide8.data.int(), wide4.data.int()
+    for make, match in ((lambda: lowp.LowpLinearPlan(a8, floats, d), "w data"),
+                        (lambda: lowp.LowpLinearPlan(a8, doubles, d), "w scales"),
+                        (lambda: lowp.LowpLinearPlan(a4, words, d), "w atoms"),
+                        (lambda: lowp.LowpLinearPlan(wide4, b4, d), "x data"),
+                        (lambda: quantize.RmsNormFp8Plan(x, torch.ones(128), wide8), "out.data"),
+                        (lambda: quantize.Fp4QuantPlan(x, wide4), "out.data"),
+                        (lambda: lowp.LowpLinearPlan(a8, b8, d), "CUDA"),
+                        (lambda: lowp.LowpLinearPlan(a4, b4, d), "CUDA")):
+        with pytest.raises(ValueError, match=match):
+            make()
+
+
 def test_native_refusals(lib):
     """The C entries refuse bad arguments before they look for a device."""
     plan = ctypes.c_void_p()
