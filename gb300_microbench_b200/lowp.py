@@ -70,7 +70,7 @@ def nvfp4_quantize(x: torch.Tensor, tensor_scale: float | None = None) -> tuple[
     x = x.float()
     r, k = x.shape
     if tensor_scale is None:
-        amax = float(x.abs().max())
+        amax = float(x.abs().max()) if x.numel() else 0.0
         gscale = amax / (E4M3_MAX * E2M1_MAX) if amax > 0 else 1.0
         if torch.tensor(gscale, dtype=torch.float32) == 0:  # below FP32: everything rounds to zero
             gscale = 1.0

@@ -117,6 +117,13 @@ def test_fp8_blocks_below_the_scales_range():
     assert ((got - x.double()).abs() <= x.double().abs() * 2.0 ** -4 + 448 * 2.0 ** -150 + 2.0 ** -150).all()
 
 
+@pytest.mark.parametrize("make", [lowp.Nvfp4Operand, lowp.Mxfp4Operand, lowp.Fp8GroupOperand, lowp.Fp8BlockOperand])
+def test_operands_of_no_rows(make):
+    op = make(torch.empty(0, 256))
+    assert (op.rows, op.k) == (0, 256) and op.data.shape[0] == 0
+    assert op.to("cpu").dequantize().shape == (0, 256)
+
+
 @pytest.mark.parametrize("rows,width", [(1, 1), (130, 5), (128, 8), (257, 90)])
 def test_scale_atoms_round_trip(rows, width):
     s = torch.randint(0, 256, (rows, width), dtype=torch.uint8, generator=torch.Generator().manual_seed(rows))
