@@ -41,8 +41,9 @@ constexpr int kMaxSplits = 8;  // the portable cluster size
 // 2880 8.8 and 10.2): their scales are the tensor core's.
 //
 // What bounds it is the weight stream, and then the ends of the launch: two
-// CTAs of up to 113 KiB share an SM (all but the turned tiles), so about 200 KiB
-// of weights per SM are in flight, and CTAs of the next launch start beside the
+// CTAs of up to 113 KiB share an SM (all but the turned tiles), so 96 to 160 KiB
+// of weights per SM are in flight (16 KiB for each of FewCfg::STAGES; 160 for FP8
+// and MXFP4 with 16 tokens), and CTAs of the next launch start beside the
 // last ones of this, set up, and fetch their first weights into L2. (A load
 // balanced to the row, by tiles of 97 instead of 128 weight rows and so two
 // CTAs on every SM, was slower: FP8 1 x 14336 x 4096 14.3 us against 13.0. It

@@ -9,8 +9,9 @@
 //     MXFP4: b = 2^(floor(log2 amax_32) - 2) as E8M0, q = e2m1(x / b)
 //     with the scales stored as the 512-byte atoms the tensor core reads.
 //
-// Both read each input once and are bound by DRAM bandwidth at large sizes and
-// by launch latency at small ones. All statistics are FP32. The only
+// Each input is read once, except where an NVFP4 tensor scale is to be found: x is
+// then read a second time, and of a few rows by every CTA. They are bound by DRAM
+// bandwidth at large sizes and by launch latency at small ones. All statistics are FP32. The only
 // roundings to fewer bits are the ones in the formulas: the stored h (the next
 // layer reads it, so the norm is of the stored value), the scales of the 4-bit
 // formats and the values themselves.

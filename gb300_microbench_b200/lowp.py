@@ -640,13 +640,17 @@ class LowpLinearPlan:
         return 2 * self.m * self.n * self.k
 
     def run(self, iterations: int = 1) -> None:
-        """`iterations` back-to-back launches on the plan's stream (async)."""
+        """`iterations` back-to-back launches on the plan's stream (async). A
+        device-side wait that times out ends its launch without an error here;
+        :meth:`synchronize` reports it, and until then later launches of the
+        plan give up early and leave D undefined."""
         status = self._execute(self._handle, int(iterations))
         if status:
             nat.check("bb_linear_execute_n", status)
 
     def synchronize(self) -> None:
-        """Waits for the stream; raises on a device-side wait timeout."""
+        """Waits for the stream; raises on a device-side wait timeout (the plan
+        is then to be closed)."""
         nat.check("bb_linear_synchronize", self._lib.bb_linear_synchronize(self._handle))
 
     @property

@@ -5,9 +5,12 @@ and the 4-bit microscaled formats. They fill the operands that
 Like the GEMM plans, a plan is built once for fixed tensors and run many
 times on its stream; the tensors stay the caller's, and x may hold new data at
 every run. Runs can be captured into a CUDA graph, which then needs the plan
-(and its tensors) to stay alive; a plan's runs belong to one stream at a time. ``lowp.nvfp4_quantize``, ``lowp.mxfp4_quantize`` and
+(and its tensors) to stay alive; a plan's runs belong to one stream at a time.
+``lowp.nvfp4_quantize``, ``lowp.mxfp4_quantize`` and
 ``lowp.fp8_group_quantize`` are the same formats in torch; the 4-bit
 kernels equal them bit for bit (on the CPU, where torch divides exactly).
+Plans are made outside a capture (making one may allocate), and run on their own
+stream whatever the current one is.
 """
 from __future__ import annotations
 
