@@ -90,7 +90,7 @@ class RmsNormFp8Plan(_QuantPlan):
     h (it may be ``residual`` or ``x``; by default the sum is not stored).
     ``weight`` is (cols,), of x's dtype or float32. cols is at most 65536;
     rows may be 0. Finite rows are right up to the ends of x's range, where
-    squares leave FP32's. A row that holds a NaN is NaN, scales and codes. In one
+    squares leave FP32's (y itself must lie inside). A row that holds a NaN is NaN, scales and codes. In one
     that holds an infinity the formula gives NaN for its 128 columns and, as
     1 / rms is 0, codes 0 with scale 1 for the others: a product's row of either
     is NaN. With eps = 0 a row of zeros is NaN (0 / 0)."""

@@ -352,7 +352,8 @@ BB_API int bb_fp4_quant_plan_create(int format, int64_t rows, int64_t cols, cons
  * rsqrt(mean(h^2) + eps) * weight; q = E4M3 of y / s (row stride q_ld) with s =
  * max|y| / 448 over each 128 columns (1 where that is 0 in FP32), stored to
  * scales[group * scales_ld + row]. cols up to 65536; weight is FP32 or of x's
- * dtype. Finite rows are right up to the ends of x's range. A row with a NaN is
+ * dtype. Finite rows are right up to the ends of x's range, as long as y lies in
+ * FP32's. A row with a NaN is
  * NaN; in one with an infinity the 128 columns around it are NaN and the others
  * 0 with scale 1 (1 / rms is 0); with eps 0 a row of zeros is NaN. */
 BB_API int bb_rmsnorm_fp8_plan_create(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t x_ld,

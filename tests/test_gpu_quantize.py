@@ -105,6 +105,30 @@ def test_norm_zero_and_non_finite_rows(cuda_device):
     assert torch.isnan(q[3, 5]) and torch.isnan(s[3, 0])
 
 
+def _round_once(x, dtype):
+    """FP64 to the nearest number of a 16-bit type, ties to even. (Tensor.to goes by way of FP32.)"""
+    digits, least = (8, -133) if dtype == torch.bfloat16 else (11, -24)
+    step = torch.exp2((torch.frexp(x).exponent - digits).clamp(min=least).double())
+    return (torch.round(x / step) * step).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols", [4096, 4095])
+def test_norm_sums_of_every_magnitude(cuda_device, dtype, cols):
+    """h is x + residual rounded once, to the bit: all finite patterns, subnormal numbers and signed zeros
+    among them, with sums at every distance of exponents."""
+    g = torch.Generator().manual_seed(10)
+    bits = [torch.randint(-2 ** 15, 2 ** 15, (64, cols), generator=g).to(torch.int16) for _ in range(2)]
+    near = torch.randint(-2 ** 10, 2 ** 10, (32, cols), generator=g).to(torch.int16)  # exponents close by
+    bits[1][:32] = bits[0][:32] ^ near
+    bits[0][40:48] &= 0xFF  # subnormal and small numbers
+    bits[1][44:52] &= 0x1FF
+    x, res = (torch.where(torch.isfinite(b.view(dtype).float()), b, 0).view(dtype) for b in bits)
+    h, _, _ = _norm(x, torch.ones(cols), cuda_device, res)
+    want = _round_once(x.double() + res.double(), dtype)
+    assert torch.equal(h.view(torch.int16), want.view(torch.int16))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("cols", [640, 637])
 def test_norm_infinite_rows(cuda_device, dtype, cols):
